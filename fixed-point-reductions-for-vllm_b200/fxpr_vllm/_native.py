@@ -7,6 +7,7 @@ device, the call raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -35,6 +36,7 @@ EXPORTED = (
     "fxpr_fxp_sum", "fxpr_gemm_workspace_bytes", "fxpr_gemm_fxp", "fxpr_fixed_to_float_bias",
     "fxpr_rms_norm_fxp", "fxpr_unified_attention_fxp", "fxpr_log_softmax_fxp", "fxpr_probe_prims",
     "fxpr_gemm_fxp_noalloc", "fxpr_attention_workspace_bytes", "fxpr_fixed_to_float_add_rms_norm",
+    "fxpr_qk_norm_rope_fxp", "fxpr_rope_append_kv_fxp",
 )
 
 _i = ctypes.c_int
@@ -67,6 +69,30 @@ class AttentionParams(ctypes.Structure):
     ]
 
 
+class RopeParams(ctypes.Structure):
+    """Mirror of ``fxpr_rope_params``."""
+
+    _fields_ = [
+        ("q", _p), ("k", _p), ("v", _p), ("dtype", _i),
+        ("q_stride_tok", _i64), ("q_stride_head", _i64), ("k_stride_tok", _i64),
+        ("k_stride_head", _i64), ("v_stride_tok", _i64), ("v_stride_head", _i64),
+        ("q_out", _p), ("qo_stride_tok", _i64), ("qo_stride_head", _i64),
+        ("k_out", _p), ("ko_stride_tok", _i64), ("ko_stride_head", _i64),
+        ("q_weight", _p), ("k_weight", _p), ("weight_dtype", _i),
+        ("positions", _p), ("positions_64", _i),
+        ("table", _p), ("table_dtype", _i), ("table_rows", _i64), ("table_stride", _i64),
+        ("rot_dim", ctypes.c_int32), ("is_neox", ctypes.c_int32),
+        ("k_cache", _p), ("v_cache", _p), ("cache_dtype", _i),
+        ("kc_stride_blk", _i64), ("kc_stride_slot", _i64), ("kc_stride_head", _i64),
+        ("vc_stride_blk", _i64), ("vc_stride_slot", _i64), ("vc_stride_head", _i64),
+        ("num_blocks", _i64), ("page_size", ctypes.c_int32),
+        ("slot_mapping", _p), ("num_slots", _i64), ("tokens", _i64),
+        ("num_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("eps", _f),
+        ("frac_bits", ctypes.c_int32), ("int_bits", ctypes.c_int32),
+    ]
+
+
 _SIGS = {
     "fxpr_abi_version": (_i, []),
     "fxpr_last_error": (ctypes.c_char_p, []),
@@ -86,6 +112,8 @@ _SIGS = {
     "fxpr_unified_attention_fxp": (_i, [ctypes.POINTER(AttentionParams), _p]),
     "fxpr_attention_workspace_bytes": (_i64, [ctypes.POINTER(AttentionParams)]),
     "fxpr_log_softmax_fxp": (_i, [_p, _i64, _p, _i64, _i64, _i64, _i, _i, _p]),
+    "fxpr_qk_norm_rope_fxp": (_i, [ctypes.POINTER(RopeParams), _p]),
+    "fxpr_rope_append_kv_fxp": (_i, [ctypes.POINTER(RopeParams), _p]),
     "fxpr_probe_prims": (_i, [_i, _p, _p, _p, _i64, _p]),
 }
 
@@ -138,6 +166,22 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
             raise RuntimeError("fxpr_vllm kernels require CUDA tensors (no CPU fallback)")
         dev = t.device if dev is None else dev
     return dev
+
+
+def same_device(*tensors: torch.Tensor | None) -> torch.device:
+    """The one CUDA device of all given tensors; raises if there are several."""
+    dev = require_cuda(*tensors)
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def on_device(device: torch.device):
+    """Context in which kernels launch on ``device``, whichever device is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def stream_ptr(device: torch.device) -> int:

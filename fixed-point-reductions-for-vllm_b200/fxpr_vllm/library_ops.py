@@ -8,8 +8,8 @@ The three reference schemas are registered unchanged in namespace ``fxpr``:
 
 plus the ops this build adds (integer GEMM partials for the tensor-parallel
 integer allreduce, its epilogue, the casts, the row sum, attention,
-log-softmax, and the rotary position with the per-head norm or the
-paged-cache append). Each has a CUDA implementation only (calls into the C ABI on
+log-softmax, the rotary position with the per-head norm or the paged-cache
+append, and the verification of drafted tokens). Each has a CUDA implementation only (calls into the C ABI on
 the current stream, no host sync) and a fake implementation for tracing;
 there is no CPU implementation, so CPU tensors fail loudly.
 """
@@ -24,6 +24,7 @@ from .fixed_point_kernels import gemm as _gemm
 from .fixed_point_kernels import rms_norm as _rms
 from .fixed_point_kernels import rope as _rope
 from .fixed_point_kernels import softmax as _sm
+from .fixed_point_kernels import verify as _verify
 
 
 @torch.library.custom_op("fxpr::gemm_fxp", mutates_args=(), device_types="cuda")
@@ -183,3 +184,17 @@ _register(
     "float eps, int frac_bits, int fxp_int_bits) -> Tensor",
     _rope.rope_append_kv_fxp,
     lambda q, *_: q.new_empty(q.shape))
+
+
+def _verify_fake(target_probs, draft_probs, draft_token_ids, draft_start_loc, bonus_token_ids, accept_uniform,
+                 resample_uniform, max_draft_len, frac_bits):
+    n = bonus_token_ids.shape[0]
+    return (target_probs.new_empty((n, max_draft_len + 1), dtype=torch.int32),
+            target_probs.new_empty((n,), dtype=torch.int32))
+
+
+_register(
+    "verify_draft_fxp(Tensor target_probs, Tensor? draft_probs, Tensor draft_token_ids, Tensor draft_start_loc, "
+    "Tensor bonus_token_ids, Tensor accept_uniform, Tensor resample_uniform, int max_draft_len, int frac_bits) "
+    "-> (Tensor, Tensor)",
+    _verify.verify_draft_fxp, _verify_fake)

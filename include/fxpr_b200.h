@@ -231,6 +231,30 @@ int fxpr_qk_norm_rope_fxp(const fxpr_rope_params* p, void* stream);
  * of two tokens with one slot, each value comes from either of them. */
 int fxpr_rope_append_kv_fxp(const fxpr_rope_params* p, void* stream);
 
+/* Verification of drafted tokens in integers. Request r has the drafted
+ * positions i in [draft_start_loc[r], draft_start_loc[r + 1]) (at most
+ * max_draft_len of them are looked at), rows i of target_probs and draft_probs
+ * [num_drafts, vocab]. With P and Q the probabilities clamped to [0, 1] and
+ * rounded to the 2^-frac_bits grid (NaN = 0), and random numbers truncated to
+ * 24 bits: token x is taken iff u * Q(x) < P(x); at the first position that is
+ * not, a token is drawn from max(P - Q, 0) (from P where that is zero
+ * everywhere) as the smallest v whose running sum exceeds
+ * floor(resample * total); when all are taken the request's bonus token
+ * follows. draft_probs NULL: a deterministic drafter, Q = 1 at the drafted
+ * token. token_ids [num_requests, max_draft_len + 1] int32 get the taken
+ * tokens, the drawn or bonus token, then -1; num_accepted the number taken.
+ * A drafted id outside the vocabulary is not taken; a position outside
+ * [0, num_drafts), or one whose target row is zero everywhere, draws -1.
+ * max_draft_len <= 32, frac_bits 1..30, vocab <= 2^24. No counterpart in the
+ * reference. */
+int fxpr_verify_draft_fxp(const void* target_probs, const void* draft_probs, int probs_dtype,
+                          int64_t target_row_stride, int64_t draft_row_stride, int64_t num_drafts,
+                          int64_t vocab, const void* draft_token_ids, int draft_ids_64,
+                          const int32_t* draft_start_loc, const void* bonus_token_ids, int bonus_ids_64,
+                          const float* accept_uniform, const float* resample_uniform,
+                          int64_t num_requests, int max_draft_len, int frac_bits, int32_t* token_ids,
+                          int64_t out_row_stride, int32_t* num_accepted, void* stream);
+
 /* Test hook: evaluates on the device the fp32 primitives the kernels use
  * where the reference relies on the GPU compiler's rounding. op: 0 exp2(a),
  * 1 a / b (fast divide), 2 sqrt(a) (fast), 3 tanh(a), 4 exp(a), 5 log(a). */

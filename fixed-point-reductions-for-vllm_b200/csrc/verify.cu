@@ -18,9 +18,9 @@
 // chain of dependent reads for a few requests. One cluster of CTAs per
 // request: every CTA decides on the drafted tokens by itself (one lane per
 // position), then sums its slice of the vocabulary; the slices' sums meet in
-// distributed shared memory, and the CTA that holds the goal finds the token
-// among its warps' sums and re-reads one warp's share from L2. Nothing is
-// read for a request whose drafts are all taken.
+// distributed shared memory, and the CTA that holds the goal finds the token:
+// the warp whose share it lies in, then that share again from L2, a turn per
+// warp. Nothing is read for a request whose drafts are all taken.
 #include <cooperative_groups.h>
 
 #include "fxp_common.cuh"
@@ -30,7 +30,12 @@ namespace cg = cooperative_groups;
 namespace fxpr {
 namespace verify {
 
-constexpr int THREADS = 512;
+// 256 threads, six CTAs per SM (40 registers), four loads of a lane in flight: 128 requests of 128256 fp32 entries, 81 of them
+// refusing (83 MB), 24.1 us (3.5 TB/s, 53% of a copy, of which about 8 us are the launch, the chain of reads that decides on
+// the drafted tokens, and the draw). 512 threads 24.8 to 31 us; fewer resident CTAs 35 us. One request: 4.7 us.
+constexpr int THREADS = 256;
+constexpr int MINB = 6;
+constexpr int UNROLL = 4;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_DRAFTS = 32;  // one lane per drafted position
 constexpr int MAX_CLUSTER = 8;
@@ -59,7 +64,7 @@ struct Params {
 
 // F2X of a probability: 0 for NaN and below 0, 2^f from 1 on; exact scaling, one rounding
 __device__ __forceinline__ uint32_t grid_of(float x, float scale) {
-  return __float2uint_rn(__fmul_rn(fminf(fmaxf(x, 0.0f), 1.0f), scale));
+  return __float2uint_rn(__fmul_rn(__saturatef(x), scale));
 }
 // random number in [0, 1) on the 2^-24 grid (truncated; NaN 0)
 __device__ __forceinline__ uint32_t draw_of(float x) {
@@ -77,7 +82,7 @@ __device__ __forceinline__ uint32_t left_of(T pv, T qv, int64_t v, int64_t token
   if (all) return P;
   if constexpr (Q) {
     const uint32_t D = grid_of(to_f32(qv), scale);
-    return P > D ? P - D : 0u;
+    return max(P, D) - D;
   } else {
     return v == token ? 0u : P;
   }
@@ -85,15 +90,34 @@ __device__ __forceinline__ uint32_t left_of(T pv, T qv, int64_t v, int64_t token
 
 template <typename T, int E> struct alignas(sizeof(T) * E) Vec { T v[E]; };
 
-// E consecutive entries per load (16 bytes when rows are aligned, else one)
+// A row of the vocabulary seen from the 16-byte boundary at or before its
+// first entry: entry v is element v + shift of `base`, and element blocks of
+// E are aligned. Blocks that reach outside the row are read entry by entry.
+template <typename T, int E> struct Row {
+  const T* base;
+  __device__ __forceinline__ Vec<T, E> load(int64_t w, int64_t first, int64_t end) const {
+    Vec<T, E> x = {};
+    if (w >= first && w + E <= end) {
+      x = *reinterpret_cast<const Vec<T, E>*>(base + w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (w + e >= first && w + e < end) x.v[e] = base[w + e];
+    }
+    return x;
+  }
+};
+
+// E consecutive entries per load: 16 bytes, or one entry where the rows of the
+// two tensors lie differently to 16-byte boundaries
 template <typename T, bool Q, int E>
-__global__ void __launch_bounds__(THREADS) verify_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, MINB) verify_kernel(const __grid_constant__ Params p) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t req = blockIdx.x / ranks;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const float scale = ldexpf(1.0f, p.frac);
-  __shared__ u64 warp_sum[WARPS];
+  __shared__ u64 warp_sum[WARPS], turn_sum[WARPS];
   __shared__ u64 cta_sum;  // read by the other CTAs of the cluster
   __shared__ int s_taken;
   __shared__ bool s_refused;
@@ -136,19 +160,32 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(const __grid_constant__
   const bool exists = row >= 0 && row < p.total;
   const int64_t token = exists ? load_id(p.ids, p.ids64, row) : -1;
   const T* pr = reinterpret_cast<const T*>(p.p) + (exists ? row : 0) * p.p_stride;
-  const T* qr = Q ? reinterpret_cast<const T*>(p.q) + (exists ? row : 0) * p.q_stride : nullptr;
+  const int shift = E == 1 ? 0 : (int)((uintptr_t)pr % (E * sizeof(T)) / sizeof(T));
+  const Row<T, E> prow = {pr - shift};
+  const Row<T, E> qrow = {Q ? reinterpret_cast<const T*>(p.q) + (exists ? row : 0) * p.q_stride - shift : nullptr};
+  const int64_t end = p.vocab + shift;  // the row's entries are elements [shift, end)
+  const int64_t mark = token >= 0 && token < p.vocab ? token + shift : -1;
 
   // ---- sums of this warp's share of the vocabulary ----
   const int64_t lo = ((int64_t)rank * WARPS + warp) * p.span;
-  const int64_t hi = exists ? min(lo + p.span, p.vocab) : lo;
+  const int64_t hi = exists ? min(lo + p.span, end) : lo;
+  auto entries = [&](int64_t w, bool all, uint32_t (&x)[E]) {
+    const Vec<T, E> a = prow.load(w, shift, end);
+    Vec<T, E> b = {};
+    if constexpr (Q) b = qrow.load(w, shift, end);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = left_of<T, Q>(a.v[e], b.v[e], w + e, mark, scale, all);
+  };
   auto sum_of = [&](bool all) -> u64 {
     u64 s = 0;
-#pragma unroll 4
-    for (int64_t v = lo + lane * E; v < hi; v += 32 * E) {  // hi - v is a multiple of E
-      Vec<T, E> a = *reinterpret_cast<const Vec<T, E>*>(pr + v), b = {};
-      if constexpr (Q) b = *reinterpret_cast<const Vec<T, E>*>(qr + v);
+#pragma unroll UNROLL
+    for (int64_t w = lo + lane * E; w < hi; w += 32 * E) {
+      uint32_t x[E];
+      entries(w, all, x);
+      // two entries are at most 2^31
 #pragma unroll
-      for (int e = 0; e < E; ++e) s += left_of<T, Q>(a.v[e], b.v[e], v + e, token, scale, all);
+      for (int e = 0; e + 1 < E; e += 2) s += x[e] + x[e + 1];
+      if (E == 1) s += x[0];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -182,41 +219,52 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(const __grid_constant__
   const u64 R = draw_of(p.r[req]);
   const u64 goal = (total >> 24) * R + (((total & 0xFFFFFFull) * R) >> 24);
 
-  // ---- the warp whose share holds the goal walks it again ----
-  for (int w = 0; w < warp; ++w) before += warp_sum[w];
-  if (goal < before || goal >= before + warp_sum[warp]) return;
+  // ---- the CTA that holds the goal looks through the share it lies in, one
+  // turn of 32 * E entries per warp ----
+  int share = -1;
   u64 run = before;
-  for (int64_t v0 = lo; v0 < hi; v0 += 32 * E) {  // uniform over the warp
-    const int64_t v = v0 + lane * E;
+  for (int w = 0; w < WARPS && share < 0; ++w) {  // uniform over the CTA
+    if (goal >= run && goal < run + warp_sum[w]) share = w;
+    else run += warp_sum[w];
+  }
+  if (share < 0) return;
+  const int64_t from = ((int64_t)rank * WARPS + share) * p.span;
+  const int turns = (int)(p.span / (32 * E));
+  for (int t0 = 0; t0 < turns; t0 += WARPS) {
     uint32_t x[E];
-    u64 mine = 0;
-    Vec<T, E> a = {}, b = {};
-    if (v < hi) {
-      a = *reinterpret_cast<const Vec<T, E>*>(pr + v);
-      if constexpr (Q) b = *reinterpret_cast<const Vec<T, E>*>(qr + v);
-    }
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] = v < hi ? left_of<T, Q>(a.v[e], b.v[e], v + e, token, scale, all) : 0u;
-      mine += x[e];
-    }
+    for (int e = 0; e < E; ++e) x[e] = 0u;
+    const int64_t w = from + ((int64_t)(t0 + warp) * 32 + lane) * E;
+    if (t0 + warp < turns) entries(w, all, x);  // beyond the row: 0
+    u64 mine = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine += x[e];
     u64 upto = mine;  // over the lanes up to this one
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const u64 s = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += s;
     }
-    const uint32_t past = __ballot_sync(0xffffffffu, run + upto > goal);
-    if (past) {
-      if (lane == __ffs(past) - 1) {
-        u64 s = run + upto - mine;
-        int e = 0;
-        while (e < E - 1 && s + x[e] <= goal) s += x[e++];
-        p.out[req * p.out_stride + s_taken] = (int32_t)(v + e);
-      }
-      return;
+    if (lane == 31) turn_sum[warp] = upto;
+    __syncthreads();
+    u64 at = run;  // in front of this warp's turn
+    for (int i = 0; i < WARPS; ++i) {
+      if (i < warp) at += turn_sum[i];
+      run += turn_sum[i];
     }
-    run += __shfl_sync(0xffffffffu, upto, 31);
+    if (goal >= at + upto - mine && goal < at + upto) {  // one lane of the CTA
+      u64 s = at + upto - mine;
+      int e = 0;
+#pragma unroll
+      for (int i = 0; i < E - 1; ++i)
+        if (e == i && s + x[i] <= goal) {
+          s += x[i];
+          ++e;
+        }
+      p.out[req * p.out_stride + s_taken] = (int32_t)(w + e - shift);
+    }
+    if (goal < run) return;  // uniform over the CTA
+    __syncthreads();  // turn_sum is read
   }
 }
 
@@ -225,11 +273,12 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(const __grid_constant__
 // ---------------------------------------------------------------------------
 template <typename T, bool Q, int E>
 static int launch(Params p, int64_t requests, cudaStream_t st) {
-  // CTAs per request: enough for about two per SM over the batch, each with
-  // at least one full turn of its warps
+  // CTAs per request: what is resident at once over the batch, or somewhat
+  // more, since requests that refuse nothing leave early (two per SM 44 us,
+  // eight 24 us at the batch above); each with at least one turn of its warps
   int ranks = MAX_CLUSTER;
-  while (ranks > 1 && (requests * ranks > 2 * num_sms() || (int64_t)(ranks / 2) * THREADS * E >= p.vocab)) ranks /= 2;
-  p.span = cdiv(cdiv(p.vocab, (int64_t)ranks * WARPS), 32 * E) * 32 * E;
+  while (ranks > 1 && (requests * ranks > 8 * num_sms() || (int64_t)(ranks / 2) * THREADS * E >= p.vocab)) ranks /= 2;
+  p.span = cdiv(cdiv(p.vocab + E, (int64_t)ranks * WARPS), 32 * E) * 32 * E;  // the shift is below E
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(requests * ranks));
   cfg.blockDim = dim3(THREADS);
@@ -247,8 +296,8 @@ static int launch(Params p, int64_t requests, cudaStream_t st) {
 template <typename T>
 static int pick(const Params& p, int64_t requests, cudaStream_t st) {
   constexpr int E = 16 / (int)sizeof(T);
-  const bool vec = p.vocab % E == 0 && (uintptr_t)p.p % 16 == 0 && p.p_stride % E == 0 &&
-                   (p.q == nullptr || ((uintptr_t)p.q % 16 == 0 && p.q_stride % E == 0));
+  // rows of both tensors at the same offset from a 16-byte boundary
+  const bool vec = p.q == nullptr || ((uintptr_t)p.p % 16 == (uintptr_t)p.q % 16 && (p.p_stride - p.q_stride) % E == 0);
   if (p.q != nullptr) return vec ? launch<T, true, E>(p, requests, st) : launch<T, true, 1>(p, requests, st);
   return vec ? launch<T, false, E>(p, requests, st) : launch<T, false, 1>(p, requests, st);
 }

@@ -214,6 +214,22 @@ def test_strides_types_stream_and_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_off_the_boundary(dtype):
+    """Rows that start anywhere, alike in both tensors and not, next to values that must not be read as entries."""
+    args = _batch([3] * 6, 1111, dtype, seed=6)
+    want = _definition(*args, 3, 30)
+    n = args[0].shape[0]
+    for a, b, wa, wb in ((1, 1, 1117, 1117), (3, 3, 1120, 1128), (2, 5, 1117, 1117), (7, 7, 1120, 1121)):
+        p, q = (torch.full((n, w), 1.0, dtype=dtype, device="cuda") for w in (wa, wb))
+        pv, qv = p[:, a:a + 1111], q[:, b:b + 1111]
+        pv.copy_(args[0])
+        qv.copy_(args[1])
+        got = V.verify_draft_fxp(pv, qv, *(x.cuda() for x in args[2:]), 3)
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+@pytest.mark.gpu
 def test_large_vocabulary():
     """2^18 + 3 entries and a flat distribution: the running sum passes 32 bits."""
     v = (1 << 18) + 3

@@ -728,29 +728,7 @@ Plan plan_of(const fxpr_attention_params* a) {
   return pl;
 }
 
-}  // namespace
-
-extern "C" int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* a) {
-  if (validate(a) != FXPR_OK) return 0;
-  if (a->num_requests <= 0 || a->max_query_len <= 0) return 0;
-  return plan_of(a).total;
-}
-
-extern "C" int fxpr_unified_attention_fxp(const fxpr_attention_params* a, void* stream) {
-  const int rc = validate(a);
-  if (rc != FXPR_OK) return rc;
-  const int D = a->head_dim;
-  const int es = elem_size(a->kv_dtype);
-  const bool aligned = ((uintptr_t)a->k_cache % 16 == 0) && ((uintptr_t)a->v_cache % 16 == 0) &&
-                       ((a->k_stride_blk * es) % 16 == 0) && ((a->k_stride_slot * es) % 16 == 0) &&
-                       ((a->k_stride_head * es) % 16 == 0) && ((a->v_stride_blk * es) % 16 == 0) &&
-                       ((a->v_stride_slot * es) % 16 == 0) && ((a->v_stride_head * es) % 16 == 0);
-  if (!aligned) {
-    set_error("unified_attention_fxp: KV cache rows must be 16-byte aligned");
-    return FXPR_ERR_INVALID;
-  }
-  if (a->num_requests <= 0 || a->max_query_len <= 0) return FXPR_OK;
-  const Plan pl = plan_of(a);
+attn::Params params_of(const fxpr_attention_params* a, const Plan& pl) {
   attn::Params p = {};
   p.q = a->q; p.q_dtype = a->q_dtype; p.q_st = a->q_stride_tok; p.q_sh = a->q_stride_head;
   p.k = a->k_cache; p.v = a->v_cache;
@@ -771,6 +749,110 @@ extern "C" int fxpr_unified_attention_fxp(const fxpr_attention_params* a, void* 
   p.page_shift = -1;
   for (int sh = 0; sh < 31; ++sh)
     if ((1 << sh) == a->page_size) p.page_shift = sh;
+  return p;
+}
+
+int check_alignment(const fxpr_attention_params* a) {
+  const int es = elem_size(a->kv_dtype);
+  const bool aligned = ((uintptr_t)a->k_cache % 16 == 0) && ((uintptr_t)a->v_cache % 16 == 0) &&
+                       ((a->k_stride_blk * es) % 16 == 0) && ((a->k_stride_slot * es) % 16 == 0) &&
+                       ((a->k_stride_head * es) % 16 == 0) && ((a->v_stride_blk * es) % 16 == 0) &&
+                       ((a->v_stride_slot * es) % 16 == 0) && ((a->v_stride_head * es) % 16 == 0);
+  if (!aligned) {
+    set_error("unified_attention_fxp: KV cache rows must be 16-byte aligned");
+    return FXPR_ERR_INVALID;
+  }
+  return FXPR_OK;
+}
+
+// ---------------------------------------------------------------------------
+// shared prefix: which calls take the prefix kernels, and their workspace
+// ---------------------------------------------------------------------------
+#ifndef FXPR_PREFIX_MIN_ROWS
+#define FXPR_PREFIX_MIN_ROWS 1
+#endif
+#ifndef FXPR_PREFIX_MIN_KEYS
+#define FXPR_PREFIX_MIN_KEYS 64
+#endif
+constexpr int kPrefixMinRows = FXPR_PREFIX_MIN_ROWS;
+constexpr int kPrefixMinKeys = FXPR_PREFIX_MIN_KEYS;
+constexpr int64_t kPrefixScores = 64ll << 20;
+
+struct PrefixPlan {
+  bool use;
+  int key0, row_tile, tiles, pass_tiles, nchunk;
+  Plan pl;
+  int64_t off_max, off_den, off_acc, off_s, off_p, total;
+};
+
+PrefixPlan prefix_plan_of(const fxpr_attention_params* a, int prefix_len, int64_t tokens) {
+  PrefixPlan pp = {};
+  pp.pl = plan_of(a);
+  const Plan& pl = pp.pl;
+  auto half = [](int d) { return d == FXPR_F16 || d == FXPR_BF16; };
+  int key0 = prefix_len < pl.max_keys ? prefix_len : pl.max_keys;
+  key0 = key0 / attn::KT * attn::KT;  // the last keys of a ragged prefix run with each request's own
+  const int64_t rows_kv = tokens * pl.G;
+  if ((a->head_dim != 64 && a->head_dim != 128) || !half(a->q_dtype) || !half(a->kv_dtype) ||
+      key0 < kPrefixMinKeys || rows_kv < kPrefixMinRows || a->num_blocks <= 0)
+    return pp;
+  pp.key0 = key0;
+  pp.row_tile = rows_kv <= 16 ? 16 : rows_kv <= 32 ? 32 : 64;
+  const int64_t tiles = cdiv(rows_kv, pp.row_tile);
+  pp.nchunk = (int)cdiv(pl.max_keys - key0, attn::CHUNK);
+  if (pp.nchunk < 1) pp.nchunk = 1;
+  const int64_t rows = tokens * a->num_heads;
+  const int64_t tile_bytes = (int64_t)a->num_kv_heads * pp.row_tile * key0 * 4;
+  int64_t pass = kPrefixScores / tile_bytes;
+  if (pass < 1) pass = 1;
+  if (pass > tiles) pass = tiles;
+  if (pass > 65535) pass = 65535;
+  if (tiles > 0x7fffffffLL || (int64_t)a->num_requests * pl.qtiles > 65535 || a->num_kv_heads > 65535 || pl.ys > 65535)
+    return pp;
+  pp.tiles = (int)tiles;
+  pp.pass_tiles = (int)pass;
+  pp.off_max = align256(pl.items * 4);
+  pp.off_den = align256(pp.off_max + rows * 4);
+  pp.off_acc = align256(pp.off_den + rows * 8);
+  pp.off_s = align256(pp.off_acc + rows * a->head_dim * 8);
+  pp.off_p = align256(pp.off_s + pl.items * pl.rp * pp.nchunk * attn::CHUNK * 4);
+  pp.total = pp.off_p + pass * tile_bytes;
+  pp.use = pp.total <= 2 * kChunkWsLimit;
+  return pp;
+}
+
+int validate_prefix(const fxpr_attention_params* a, int prefix_len, int64_t tokens) {
+  const int rc = validate(a);
+  if (rc != FXPR_OK) return rc;
+  if (a->frac_bits < 0 || a->frac_bits >= a->int_bits) {
+    set_error("shared_prefix_attention_fxp: frac_bits must satisfy 0 <= frac_bits < %d, got %d", a->int_bits, a->frac_bits);
+    return FXPR_ERR_INVALID;
+  }
+  if (prefix_len < 0 || prefix_len > (int64_t)a->block_table_cols * a->page_size || tokens < 0) {
+    set_error("shared_prefix_attention_fxp: common_prefix_len %d outside the block table's %lld keys", prefix_len,
+              (long long)a->block_table_cols * a->page_size);
+    return FXPR_ERR_INVALID;
+  }
+  return FXPR_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* a) {
+  if (validate(a) != FXPR_OK) return 0;
+  if (a->num_requests <= 0 || a->max_query_len <= 0) return 0;
+  return plan_of(a).total;
+}
+
+extern "C" int fxpr_unified_attention_fxp(const fxpr_attention_params* a, void* stream) {
+  const int rc = validate(a);
+  if (rc != FXPR_OK) return rc;
+  const int D = a->head_dim;
+  const int ra = check_alignment(a);
+  if (ra != FXPR_OK) return ra;
+  if (a->num_requests <= 0 || a->max_query_len <= 0) return FXPR_OK;
+  const Plan pl = plan_of(a);
+  attn::Params p = params_of(a, pl);
   const cudaStream_t st = (cudaStream_t)stream;
   const int R = a->num_requests;
 
@@ -814,4 +896,52 @@ extern "C" int fxpr_unified_attention_fxp(const fxpr_attention_params* a, void* 
     case 128: return attn::pick_rp<128>(p, rp, a->int_bits, a->kv_dtype, max_keys, splits, R, ys, st);
     default: return attn::pick_rp<256>(p, rp, a->int_bits, a->kv_dtype, max_keys, splits, R, ys, st);
   }
+}
+
+extern "C" int64_t fxpr_shared_prefix_attention_workspace_bytes(const fxpr_attention_params* a, int common_prefix_len,
+                                                                int64_t num_tokens) {
+  if (validate_prefix(a, common_prefix_len, num_tokens) != FXPR_OK) return 0;
+  if (a->num_requests <= 0 || a->max_query_len <= 0 || num_tokens <= 0) return 0;
+  const PrefixPlan pp = prefix_plan_of(a, common_prefix_len, num_tokens);
+  return pp.use ? pp.total : pp.pl.total;
+}
+
+extern "C" int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* a, int common_prefix_len,
+                                                int64_t num_tokens, void* stream) {
+  int rc = validate_prefix(a, common_prefix_len, num_tokens);
+  if (rc != FXPR_OK) return rc;
+  if (a->num_requests <= 0 || a->max_query_len <= 0 || num_tokens <= 0) return FXPR_OK;
+  const PrefixPlan pp = prefix_plan_of(a, common_prefix_len, num_tokens);
+  if (!pp.use || a->workspace == nullptr) return fxpr_unified_attention_fxp(a, stream);
+  rc = check_alignment(a);
+  if (rc != FXPR_OK) return rc;
+  if (a->workspace_bytes < pp.total || (uintptr_t)a->workspace % 256 != 0) {
+    set_error("shared_prefix_attention_fxp: the workspace must be 256-byte aligned and hold %lld bytes", (long long)pp.total);
+    return FXPR_ERR_INVALID;
+  }
+  const Plan& pl = pp.pl;
+  const cudaStream_t st = (cudaStream_t)stream;
+  unsigned char* ws = reinterpret_cast<unsigned char*>(a->workspace);
+  attn::Params p = params_of(a, pl);
+  p.ws_cnt = reinterpret_cast<uint32_t*>(ws);
+  p.row_max = reinterpret_cast<uint32_t*>(ws + pp.off_max);
+  p.row_den = reinterpret_cast<unsigned long long*>(ws + pp.off_den);
+  p.row_acc = reinterpret_cast<unsigned long long*>(ws + pp.off_acc);
+  p.ws_s = reinterpret_cast<float*>(ws + pp.off_s);
+  p.nchunk_max = pp.nchunk;
+  p.key0 = pp.key0;
+  float* scores = reinterpret_cast<float*>(ws + pp.off_p);
+  if (cudaMemsetAsync(ws, 0, pp.off_s, st) != cudaSuccess) return check_launch("fxpr_shared_prefix_attention_fxp (clear)");
+  rc = attn::launch_suffix(p, false, a->head_dim, pl.rp, a->int_bits, a->kv_dtype, a->num_requests, pl.ys, st);
+  // with more row tiles than the scores' workspace holds, the prefix runs in
+  // passes over the tiles (a row's maximum is complete after its own pass)
+  for (int tile = 0; rc == FXPR_OK && tile < pp.tiles; tile += pp.pass_tiles) {
+    const int n = pp.tiles - tile < pp.pass_tiles ? pp.tiles - tile : pp.pass_tiles;
+    for (int pv = 0; rc == FXPR_OK && pv < 2; ++pv)
+      rc = attn::launch_prefix(p, pv != 0, a->head_dim, pp.row_tile, a->int_bits, a->kv_dtype, a->num_requests,
+                               a->num_blocks, num_tokens, scores, tile, n, st);
+  }
+  if (rc == FXPR_OK)
+    rc = attn::launch_suffix(p, true, a->head_dim, pl.rp, a->int_bits, a->kv_dtype, a->num_requests, pl.ys, st);
+  return rc;
 }

@@ -198,7 +198,8 @@ __device__ __forceinline__ float score_of(const Params& p, long long di, int j, 
 // kernel 1 (general shapes): scores and chunk row maxima. Four threads share
 // a key (each a quarter of its dims), q read from shared memory.
 // ---------------------------------------------------------------------------
-template <int D, int RP, int BITS, typename KVT, bool PL>
+// PRE: the shared-prefix form, over the keys from p.key0 on.
+template <int D, int RP, int BITS, typename KVT, bool PL, bool PRE = false>
 __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
   using TL = Tile<D, KVT>;
   using SM = ScoreSmem<D, RP, KVT>;
@@ -222,9 +223,11 @@ __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
   const int kvh = blockIdx.y / p.head_slices, hslice = blockIdx.y % p.head_slices;
   const int req = blockIdx.z / p.qtiles, qtile = blockIdx.z % p.qtiles;
   if (t == 0) q_or = 0u;
-  const int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
-  const int kb = chunk * CHUNK;
-  if (kr_hi < 0 || (chunk > 0 && kb >= kr_hi)) return;  // uniform over the CTA
+  int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
+  if (kr_hi < 0) return;  // uniform over the CTA
+  if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
+  const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
+  if (chunk > 0 && kb >= kr_hi) return;
   const int ke = min(kb + CHUNK, kr_hi);
   const int ntiles = (ke - kb + KT - 1) / KT;
   const int64_t item = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
     cp_async_commit();
   }
   int next_blk = (NBS - 1 < ntiles) ? cp.block_of(NBS - 1) : -1;
-  clear_item<RP, D>(p, item, chunk, kr_hi);
+  if constexpr (!PRE) clear_item<RP, D>(p, item, chunk, kr_hi);
   const float kthr = stage_q<RP, D>(p, row_tok, row_head, q_s, q_raw, &q_or, scale);
 
   float* sdst = p.ws_s + unit * (RP * CHUNK);
@@ -372,7 +375,11 @@ __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) m = fmaxf(m, wmax[w][t]);
-    p.ws_m[unit * RP + t] = m;
+    if constexpr (PRE) {
+      if (row_tok[t] >= 0) atomicMax(&p.row_max[(int64_t)row_tok[t] * p.num_heads + row_head[t]], ordered(m));
+    } else {
+      p.ws_m[unit * RP + t] = m;
+    }
   }
 }
 
@@ -383,7 +390,7 @@ __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
 // once and q never is; the 8 partial dots of (2 keys x 4 rows) are
 // reduce-scattered over the 8 lanes, one score per lane.
 // ---------------------------------------------------------------------------
-template <int D, int BITS, typename KVT, bool PL>
+template <int D, int BITS, typename KVT, bool PL, bool PRE = false>
 __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
   constexpr int RP = 4;
   using TL = Tile<D, KVT, KTC>;
@@ -413,9 +420,11 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
   const int kvh = blockIdx.y / p.head_slices, hslice = blockIdx.y % p.head_slices;
   const int req = blockIdx.z / p.qtiles, qtile = blockIdx.z % p.qtiles;
   if (t == 0) q_or = 0u;
-  const int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
-  const int kb = chunk * CHUNK;
-  if (kr_hi < 0 || (chunk > 0 && kb >= kr_hi)) return;  // uniform over the CTA
+  int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
+  if (kr_hi < 0) return;  // uniform over the CTA
+  if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
+  const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
+  if (chunk > 0 && kb >= kr_hi) return;
   const int ke = min(kb + CHUNK, kr_hi);
   const int ntiles = (ke - kb + KTC - 1) / KTC;
   const int64_t item = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
@@ -431,7 +440,7 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
     cp_async_commit();
   }
   int next_blk = (NBS - 1 < ntiles) ? cp.block_of(NBS - 1) : -1;
-  clear_item<RP, D>(p, item, chunk, kr_hi);
+  if constexpr (!PRE) clear_item<RP, D>(p, item, chunk, kr_hi);
   const float kthr = stage_q<RP, D>(p, row_tok, row_head, q_s, q_raw, &q_or, scale);
 
   // this thread's q (pre-scaled), as fp32 pairs
@@ -618,14 +627,21 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
     float m = -INFINITY;
 #pragma unroll
     for (int w2 = 0; w2 < THREADS / 32; ++w2) m = fmaxf(m, wmax[w2][t]);
-    p.ws_m[unit * RP + t] = m;
+    if constexpr (PRE) {
+      if (row_tok[t] >= 0) atomicMax(&p.row_max[(int64_t)row_tok[t] * p.num_heads + row_head[t]], ordered(m));
+    } else {
+      p.ws_m[unit * RP + t] = m;
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
 // kernel 2: normaliser, PV and the integer combine
 // ---------------------------------------------------------------------------
-template <int D, int RP, int BITS, typename KVT>
+// PRE: over the keys from p.key0 on; the row maxima are complete, the sums of
+// the keys before are in the row accumulators, and a masked key (score -inf,
+// kept as p = -0) contributes nothing whatever its V holds.
+template <int D, int RP, int BITS, typename KVT, bool PRE = false>
 __global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
   using TL = Tile<D, KVT>;
   using SM = PvSmem<D, RP, KVT>;
@@ -649,15 +665,17 @@ __global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
   const int chunk = blockIdx.x;
   const int kvh = blockIdx.y / p.head_slices, hslice = blockIdx.y % p.head_slices;
   const int req = blockIdx.z / p.qtiles, qtile = blockIdx.z % p.qtiles;
-  const int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
-  const int kb = chunk * CHUNK;
-  if (kr_hi < 0 || (chunk > 0 && kb >= kr_hi)) return;  // uniform over the CTA
+  int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
+  if (kr_hi < 0) return;  // uniform over the CTA
+  if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
+  const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
+  if (chunk > 0 && kb >= kr_hi) return;
   const int ke = min(kb + CHUNK, kr_hi);
   const int ntiles = (ke - kb + KT - 1) / KT;
   const int nk = ntiles * KT;
   // units of this item; a context beyond the caller's max_seq_len hint is cut
   // at the workspace's capacity (nchunk_max units) instead of overrunning it
-  const int nch = min(p.nchunk_max, max(1, (kr_hi + CHUNK - 1) / CHUNK));
+  const int nch = min(p.nchunk_max, max(1, (kr_hi - (PRE ? p.key0 : 0) + CHUNK - 1) / CHUNK));
   const int64_t item = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
   const int64_t unit = item * p.nchunk_max + chunk;
   const float scale = ldexpf(1.0f, p.frac);
@@ -684,8 +702,12 @@ __global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
   if (t < RP) {
     den_s[t] = 0ull;
     float m = -INFINITY;
-    const float* mrow = p.ws_m + item * p.nchunk_max * RP + t;
-    for (int c = 0; c < nch; ++c) m = fmaxf(m, mrow[c * RP]);
+    if constexpr (PRE) {
+      if (row_tok[t] >= 0) m = from_ordered(p.row_max[(int64_t)row_tok[t] * p.num_heads + row_head[t]]);
+    } else {
+      const float* mrow = p.ws_m + item * p.nchunk_max * RP + t;
+      for (int c = 0; c < nch; ++c) m = fmaxf(m, mrow[c * RP]);
+    }
     gmax_s[t] = m;  // == the reference's pass-1 max over the whole context
   }
   cp_async_wait<NBP - 2>();  // scores and V tile 0
@@ -698,7 +720,9 @@ __global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
     const int j = kb + k;
     float pv = 0.0f;
     UAcc den = 0;
-    if (j < ke) {
+    if (PRE && (j >= ke || P_all[i * CHUNK + k] == -INFINITY)) {
+      pv = -0.0f;
+    } else if (j < ke) {
       pv = prim_exp2(__fsub_rn(P_all[i * CHUNK + k], gmax_s[i]));
       if (j < row_kend[i]) den = (UAcc)f2x_f32<BITS>(pv, scale);
     }
@@ -816,6 +840,7 @@ __global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
         for (int i = 0; i < RP; ++i) {
           if (j >= row_kend[i]) continue;
           const float ps = Pk[i * CHUNK + u];
+          if (PRE && __float_as_uint(ps) == 0x80000000u) continue;
           const auto x0 = f2x_scaled<BITS>(__fmul_rn(ps, vv.x));
           const auto x1 = f2x_scaled<BITS>(__fmul_rn(ps, vv.y));
           if constexpr (BITS == 64) {
@@ -859,6 +884,27 @@ __global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
     const float out = prim_div(af, fmaxf(df, 1.0e-6f));
     store_f32(p.o, p.o_dtype, (int64_t)row_tok[i] * p.o_st + (int64_t)row_head[i] * p.o_sh + d, out);
   };
+  if constexpr (PRE) {  // the sums meet in the row accumulators, beside those of the prefix kernels
+    auto row_of = [&](int i) -> int64_t { return (int64_t)row_tok[i] * p.num_heads + row_head[i]; };
+    if (nch > 1) {
+      for (int e = t; e < RP * D; e += THREADS)
+        if (row_tok[e / D] >= 0 && acc_s[e]) atomicAdd(&p.row_acc[row_of(e / D) * D + e % D], acc_s[e]);
+      if (t < RP && row_tok[t] >= 0 && den_s[t]) atomicAdd(&p.row_den[row_of(t)], den_s[t]);
+      __threadfence();
+      __syncthreads();
+      if (t == 0) last_s = (atomicAdd(&p.ws_cnt[item], 1u) == (unsigned)(nch - 1));
+      __syncthreads();
+      if (!last_s) return;
+      __threadfence();
+    }
+    for (int e = t; e < RP * D; e += THREADS) {
+      if (row_tok[e / D] < 0) continue;
+      unsigned long long a = __ldcg(&p.row_acc[row_of(e / D) * D + e % D]), dn = __ldcg(&p.row_den[row_of(e / D)]);
+      if (nch == 1) a += acc_s[e], dn += den_s[e / D];
+      finalize(e, a, dn);
+    }
+    return;
+  }
   if (nch == 1) {  // the unit is the whole item
     for (int e = t; e < RP * D; e += THREADS)
       if (row_tok[e / D] >= 0) finalize(e, acc_s[e], den_s[e / D]);
@@ -977,6 +1023,56 @@ static int pick_rp_chunked(const Params& p, int rp, int bits, int kv_dtype, int 
   }
   if (bits == 32) return pick_kv_chunked<D, 16, 32>(p, kv_dtype, req, ys, st);
   return pick_kv_chunked<D, 16, 64>(p, kv_dtype, req, ys, st);
+}
+
+template <int D, int RP, int BITS, typename KVT>
+static int launch_suffix_t(const Params& p, bool pv, int req, int ys, cudaStream_t st) {
+  constexpr bool rq = RP == 4;
+  const dim3 grid((unsigned)p.nchunk_max, (unsigned)ys, (unsigned)((int64_t)req * p.qtiles));
+  if (pv) {
+    static bool done[64] = {false};
+    const size_t s2 = PvSmem<D, RP, KVT>::bytes;
+    auto k2 = chunk_pv_kernel<D, RP, BITS, KVT, true>;
+    const int rc = configure((const void*)k2, s2, done);
+    if (rc != FXPR_OK) return rc;
+    k2<<<grid, THREADS, s2, st>>>(p);
+    return check_launch("fxpr_shared_prefix_attention_fxp (pv)");
+  }
+  const size_t s1 = rq ? ScoreSmem<D, RP, KVT, KTC>::bytes : ScoreSmem<D, RP, KVT>::bytes;
+  const bool plain = !(p.softcap_log2 > 0.0f) && p.alibi == nullptr && p.window <= 0;
+  void (*k1)(Params);
+  if constexpr (rq) {
+    k1 = plain ? chunk_scores_rq_kernel<D, BITS, KVT, true, true> : chunk_scores_rq_kernel<D, BITS, KVT, false, true>;
+  } else {
+    k1 = plain ? chunk_scores_kernel<D, RP, BITS, KVT, true, true> : chunk_scores_kernel<D, RP, BITS, KVT, false, true>;
+  }
+  static bool done[2][64] = {{false}};
+  const int rc = configure((const void*)k1, s1, done[plain ? 1 : 0]);
+  if (rc != FXPR_OK) return rc;
+  k1<<<grid, THREADS, s1, st>>>(p);
+  return check_launch("fxpr_shared_prefix_attention_fxp (scores)");
+}
+
+template <int D, int RP, int BITS>
+static int pick_suffix_kv(const Params& p, bool pv, int kv_dtype, int req, int ys, cudaStream_t st) {
+  if (kv_dtype == FXPR_F16) return launch_suffix_t<D, RP, BITS, __half>(p, pv, req, ys, st);
+  return launch_suffix_t<D, RP, BITS, __nv_bfloat16>(p, pv, req, ys, st);
+}
+
+template <int D>
+static int pick_suffix(const Params& p, bool pv, int rp, int bits, int kv_dtype, int req, int ys, cudaStream_t st) {
+  if (rp == 4) {
+    if (bits == 32) return pick_suffix_kv<D, 4, 32>(p, pv, kv_dtype, req, ys, st);
+    return pick_suffix_kv<D, 4, 64>(p, pv, kv_dtype, req, ys, st);
+  }
+  if (bits == 32) return pick_suffix_kv<D, 16, 32>(p, pv, kv_dtype, req, ys, st);
+  return pick_suffix_kv<D, 16, 64>(p, pv, kv_dtype, req, ys, st);
+}
+
+int launch_suffix(const Params& p, bool pv, int D, int rp, int bits, int kv_dtype, int req, int ys,
+                  cudaStream_t st) {
+  if (D == 64) return pick_suffix<64>(p, pv, rp, bits, kv_dtype, req, ys, st);
+  return pick_suffix<128>(p, pv, rp, bits, kv_dtype, req, ys, st);
 }
 
 int launch_chunked(const Params& p, int D, int rp, int bits, int kv_dtype, int req, int ys,

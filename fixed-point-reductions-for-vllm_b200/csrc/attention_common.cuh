@@ -53,7 +53,24 @@ struct Params {
   float* ws_m;                 // [items][nchunk_max][RP] chunk row maxima
   float* ws_s;                 // [items][nchunk_max][RP][CHUNK] scores
   int nchunk_max;
+  // shared-prefix form: keys before key0 belong to the prefix kernels
+  // (attention_prefix.cu); rows are token * num_heads + head
+  int key0;
+  uint32_t* row_max;            // [rows] row maxima over all keys, as ordered integers
+  unsigned long long* row_den;  // [rows] integer normaliser partial sums
+  unsigned long long* row_acc;  // [rows][D] integer PV partial sums
 };
+
+// Row maxima meet by an integer atomicMax: floats as unsigned integers of the
+// same order. 0, which memory cleared for the call holds, is below all of them.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(uint32_t u) {
+  if (u == 0u) return -INFINITY;
+  return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+}
 
 // 16-byte chunk of KV elements -> fp32 pairs
 template <typename T> struct Chunk;
@@ -140,6 +157,15 @@ int launch_decode(const fxpr_attention_params* a, int kmax, void* workspace, cud
 bool chunked_supported(int D, int rp, int kv_dtype);
 int launch_chunked(const Params& p, int D, int rp, int bits, int kv_dtype, int req, int ys,
                    cudaStream_t st);
+// the same kernels over the keys from p.key0 on, for the shared-prefix form
+// (head_dim 64 / 128, 16-bit cache): scores, or normaliser and PV
+int launch_suffix(const Params& p, bool pv, int D, int rp, int bits, int kv_dtype, int req, int ys,
+                  cudaStream_t st);
+
+// prefix kernels (attention_prefix.cu): key columns [0, p.key0) of the row
+// tiles [tile0, tile0 + tiles) of every KV head
+int launch_prefix(const Params& p, bool pv, int D, int row_tile, int bits, int kv_dtype, int num_requests,
+                  int64_t num_blocks, int64_t tokens, float* scores, int tile0, int tiles, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace fxpr

@@ -130,3 +130,101 @@ def unified_attention_fxp(
             p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     rc = lib.fxpr_unified_attention_fxp(ctypes.byref(p), N.stream_ptr(q.device))
     N.check(rc, "unified_attention_fxp")
+
+
+def shared_prefix_attention_fxp(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    o: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    seq_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    common_prefix_len: int,
+    max_query_len: int,
+    *,
+    alibi_slopes: torch.Tensor | None = None,
+    fxp_dtype=torch.int32,
+    is_causal: bool = True,
+    softmax_scale: float | None = None,
+    frac_bits: int = 16,
+    logits_soft_cap: float = 0.0,
+    window_size: int = 0,
+    max_seq_len: int | None = None,
+) -> None:
+    """:func:`unified_attention_fxp` for a batch whose requests share their
+    first ``common_prefix_len`` keys, written into ``o``: the prefix's keys and
+    values are read and converted once for a tile of rows of all requests.
+
+    The first ``common_prefix_len // page`` entries of every block-table row
+    are the same pages (those of row 0 are read), and the keys of a last page
+    that the prefix covers in part are equal in every request's own page. The
+    result has the bits of ``unified_attention_fxp``, except that a masked key
+    contributes nothing even where its V is infinite or NaN and that a row
+    which sees no key is 0. Rows of ``o`` behind ``query_start_loc[-1]`` are
+    left as they are. ``max_seq_len`` bounds every ``seq_lens`` entry when
+    given, as there. Scratch is a tensor of the call, so calls on several
+    streams and captured graphs share nothing."""
+    what = "shared_prefix_attention_fxp"
+
+    def bad(text):
+        raise ValueError(f"{what}: {text}")
+
+    if q.dim() != 3 or o.shape != q.shape:
+        bad(f"q and o must be [tokens, heads, head_dim]; got {tuple(q.shape)} and {tuple(o.shape)}")
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.shape[4] != q.shape[2]:
+        bad(f"kv_cache must be [blocks, 2, page, kv_heads, {q.shape[2]}]; got {tuple(kv_cache.shape)}")
+    tokens, heads, dim = q.shape
+    blocks, _, page, kv_heads, _ = kv_cache.shape
+    if kv_heads < 1 or heads % kv_heads != 0 or page < 1:
+        bad(f"{heads} query heads do not group over {kv_heads} KV heads, or the page is empty")
+    if block_table.dim() != 2 or seq_lens.dim() != 1 or query_start_loc.dim() != 1:
+        bad("block_table must have two dimensions, seq_lens and query_start_loc one")
+    reqs = seq_lens.shape[0]
+    if query_start_loc.shape[0] != reqs + 1 or block_table.shape[0] < reqs:
+        bad(f"{reqs} requests need {reqs + 1} query_start_loc entries and {reqs} block-table rows; got "
+            f"{query_start_loc.shape[0]} and {block_table.shape[0]}")
+    if not 0 <= common_prefix_len <= block_table.shape[1] * page:
+        bad(f"common_prefix_len {common_prefix_len} outside the block table's {block_table.shape[1] * page} keys")
+    if q.stride(2) != 1 or o.stride(2) != 1 or kv_cache.stride(4) != 1:
+        bad("head_dim must be the innermost (contiguous) dimension")
+    if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or alibi_slopes.shape != (heads,)):
+        bad(f"alibi_slopes must be float32 [{heads}] (pre-scaled by 1/ln 2)")
+    dev = N.same_device(q, kv_cache, o, query_start_loc, seq_lens, block_table, alibi_slopes)
+    if reqs == 0 or max_query_len <= 0 or tokens == 0:
+        return
+    if max_seq_len and _validate_hints() and not torch.cuda.is_current_stream_capturing():
+        check_max_seq_len_hint(seq_lens, max_seq_len)
+    qsl, sl, bt = (x.to(torch.int32) for x in (query_start_loc, seq_lens, block_table))
+    qsl, sl = qsl.contiguous(), sl.contiguous()
+    bt = bt if bt.stride(1) == 1 or bt.shape[1] == 1 else bt.contiguous()
+    slopes = alibi_slopes.contiguous() if alibi_slopes is not None else None
+    p = N.AttentionParams()
+    es, base = kv_cache.element_size(), kv_cache.data_ptr()
+    sb, s2, ss, sh, _ = kv_cache.stride()
+    p.q, p.q_dtype = q.data_ptr(), N.dcode(q)
+    p.q_stride_tok, p.q_stride_head, _ = q.stride()
+    p.k_cache, p.v_cache, p.kv_dtype = base, base + s2 * es, N.dcode(kv_cache)
+    p.k_stride_blk = p.v_stride_blk = sb
+    p.k_stride_slot = p.v_stride_slot = ss
+    p.k_stride_head = p.v_stride_head = sh
+    p.o, p.o_dtype = o.data_ptr(), N.dcode(o)
+    p.o_stride_tok, p.o_stride_head, _ = o.stride()
+    p.query_start_loc, p.seq_lens, p.block_table = qsl.data_ptr(), sl.data_ptr(), bt.data_ptr()
+    p.bt_stride, p.block_table_cols = bt.stride(0), bt.shape[1]
+    p.max_seq_len = int(max_seq_len) if max_seq_len else 0
+    p.alibi_slopes = slopes.data_ptr() if slopes is not None else None
+    p.num_requests, p.max_query_len = reqs, int(max_query_len)
+    p.num_heads, p.num_kv_heads, p.head_dim, p.page_size = heads, kv_heads, dim, page
+    p.num_blocks = blocks
+    p.is_causal, p.window_size = 1 if is_causal else 0, int(window_size)
+    p.scale_log2 = prepare_log2_softmax_scale(dim, softmax_scale)
+    p.logits_soft_cap = logits_soft_cap * RCP_LN2 if logits_soft_cap > 0.0 else 0.0
+    p.frac_bits, p.int_bits, p.num_kv_splits = frac_bits, int_bits_of(fxp_dtype), 8
+    lib = N.load()
+    with N.on_device(dev):
+        need = lib.fxpr_shared_prefix_attention_workspace_bytes(ctypes.byref(p), common_prefix_len, tokens)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        if need:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        rc = lib.fxpr_shared_prefix_attention_fxp(ctypes.byref(p), common_prefix_len, tokens, N.stream_ptr(dev))
+    N.check(rc, what)

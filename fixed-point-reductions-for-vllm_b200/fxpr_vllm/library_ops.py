@@ -9,7 +9,8 @@ The three reference schemas are registered unchanged in namespace ``fxpr``:
 plus the ops this build adds (integer GEMM partials for the tensor-parallel
 integer allreduce, its epilogue, the casts, the row sum, attention,
 log-softmax, the rotary position with the per-head norm or the paged-cache
-append, and the verification of drafted tokens). Each has a CUDA implementation only (calls into the C ABI on
+append, attention behind a shared prefix, and the verification of drafted
+tokens). Each has a CUDA implementation only (calls into the C ABI on
 the current stream, no host sync) and a fake implementation for tracing;
 there is no CPU implementation, so CPU tensors fail loudly.
 """
@@ -198,3 +199,21 @@ _register(
     "Tensor bonus_token_ids, Tensor accept_uniform, Tensor resample_uniform, int max_draft_len, int frac_bits) "
     "-> (Tensor, Tensor)",
     _verify.verify_draft_fxp, _verify_fake)
+
+
+def _shared_prefix(q, kv_cache, o, query_start_loc, seq_lens, block_table, common_prefix_len, max_query_len,
+                   alibi_slopes, fxp_int_bits, is_causal, softmax_scale, frac_bits, logits_soft_cap, window_size,
+                   max_seq_len):
+    _attn.shared_prefix_attention_fxp(q, kv_cache, o, query_start_loc, seq_lens, block_table, common_prefix_len,
+                                      max_query_len, alibi_slopes=alibi_slopes, fxp_dtype=fxp_int_bits,
+                                      is_causal=is_causal, softmax_scale=softmax_scale, frac_bits=frac_bits,
+                                      logits_soft_cap=logits_soft_cap, window_size=window_size,
+                                      max_seq_len=max_seq_len)
+
+
+_register(
+    "shared_prefix_attention_fxp(Tensor q, Tensor kv_cache, Tensor(a!) o, Tensor query_start_loc, Tensor seq_lens, "
+    "Tensor block_table, int common_prefix_len, int max_query_len, Tensor? alibi_slopes, int fxp_int_bits, "
+    "bool is_causal, float? softmax_scale, int frac_bits, float logits_soft_cap, int window_size, int max_seq_len) "
+    "-> ()",
+    _shared_prefix, lambda *_: None)

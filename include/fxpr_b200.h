@@ -175,6 +175,23 @@ int fxpr_unified_attention_fxp(const fxpr_attention_params* p, void* stream);
  * the reference has no workspace. */
 int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* p);
 
+/* fxpr_unified_attention_fxp for a batch whose requests share the first
+ * common_prefix_len keys: the block table rows of all requests start with the
+ * same common_prefix_len / page_size pages (row 0's are read) and the keys of
+ * a last, partly shared page are equal. The prefix's keys and values are read
+ * once for a tile of rows of all requests. The result has the bits of
+ * fxpr_unified_attention_fxp, except that a masked key contributes nothing
+ * even where its V is infinite or NaN, and a row that sees no key is 0.
+ * num_tokens: rows of q and o; rows behind query_start_loc[num_requests] are
+ * left as they are. num_blocks must be given; a prefix block id outside the
+ * cache reads zeros. Calls that the prefix kernels do not take (head_dim 32 or
+ * 256, a 32-bit type, a short prefix, few rows, no workspace) run the unified
+ * kernels. The workspace is 256-byte aligned, any contents. */
+int64_t fxpr_shared_prefix_attention_workspace_bytes(const fxpr_attention_params* p, int common_prefix_len,
+                                                     int64_t num_tokens);
+int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* p, int common_prefix_len, int64_t num_tokens,
+                                     void* stream);
+
 /* Row-wise log-softmax with a fixed-point exp-sum (softmax.py:8-97): logits
  * rounded to fp16 before the max and exp, [rows, n] fp32 in/out. */
 int fxpr_log_softmax_fxp(const float* x, int64_t x_row_stride, float* y, int64_t y_row_stride,

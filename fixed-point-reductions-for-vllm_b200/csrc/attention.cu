@@ -807,7 +807,7 @@ PrefixPlan prefix_plan_of(const fxpr_attention_params* a, int prefix_len, int64_
   if (pass < 1) pass = 1;
   if (pass > tiles) pass = tiles;
   if (pass > 65535) pass = 65535;
-  if (tiles > 0x7fffffffLL || (int64_t)a->num_requests * pl.qtiles > 65535 || a->num_kv_heads > 65535 || pl.ys > 65535)
+  if (rows_kv > 0x7fffffffLL - 64 || (int64_t)a->num_requests * pl.qtiles > 65535 || a->num_kv_heads > 65535 || pl.ys > 65535)
     return pp;
   pp.tiles = (int)tiles;
   pp.pass_tiles = (int)pass;

@@ -776,7 +776,7 @@ int check_alignment(const fxpr_attention_params* a) {
 #endif
 constexpr int kPrefixMinRows = FXPR_PREFIX_MIN_ROWS;
 constexpr int kPrefixMinKeys = FXPR_PREFIX_MIN_KEYS;
-constexpr int64_t kPrefixScores = 64ll << 20;
+constexpr int64_t kPrefixScores = 128ll << 20;  // about the L2
 
 struct PrefixPlan {
   bool use;
@@ -806,7 +806,7 @@ PrefixPlan prefix_plan_of(const fxpr_attention_params* a, int prefix_len, int64_
   int64_t pass = kPrefixScores / tile_bytes;
   if (pass < 1) pass = 1;
   if (pass > tiles) pass = tiles;
-  if (pass > 65535) pass = 65535;
+  pass = cdiv(tiles, cdiv(tiles, pass));  // passes of equal size
   if (rows_kv > 0x7fffffffLL - 64 || (int64_t)a->num_requests * pl.qtiles > 65535 || a->num_kv_heads > 65535 || pl.ys > 65535)
     return pp;
   pp.tiles = (int)tiles;

@@ -58,12 +58,17 @@ struct ScoreSmem {
   static constexpr size_t off_kv = off_qraw + (size_t)RP * D * 4;
   static constexpr size_t bytes = off_kv + (size_t)NBS * Tile<D, KVT, NK>::TILEB;
 };
-template <int D, int RP, typename KVT>
+template <int D, int RP, typename KVT, int NB = NBP>
 struct PvSmem {
   static constexpr size_t off_p = 0;  // [RP][CHUNK] scores, then p * 2^f
   static constexpr size_t off_kv = off_p + (size_t)RP * CHUNK * 4;
-  static constexpr size_t bytes = off_kv + (size_t)NBP * Tile<D, KVT>::TILEB;
+  static constexpr size_t bytes = off_kv + (size_t)NB * Tile<D, KVT>::TILEB;
 };
+// Resident CTAs of the shared-prefix form's PV units: four for 4-row units (64
+// requests with up to 256 own keys 21.6 us, three 25 us), one for 16-row units
+// (two would spill: 37 against 30 us).
+constexpr int NBP_PRE = 2;
+constexpr int suffix_pv_ctas(bool pre, int rp) { return pre && rp == 4 ? 4 : 1; }
 
 // Rows of a unit (attention.py:319-353). Returns the key limit over its rows
 // (the reference walks keys to the end of its 64-row query block), or -1 if
@@ -223,6 +228,7 @@ __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
   const int kvh = blockIdx.y / p.head_slices, hslice = blockIdx.y % p.head_slices;
   const int req = blockIdx.z / p.qtiles, qtile = blockIdx.z % p.qtiles;
   if (t == 0) q_or = 0u;
+  if constexpr (PRE) launch_dependents();
   int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
   if (kr_hi < 0) return;  // uniform over the CTA
   if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
@@ -642,9 +648,10 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
 // the keys before are in the row accumulators, and a masked key (score -inf,
 // kept as p = -0) contributes nothing whatever its V holds.
 template <int D, int RP, int BITS, typename KVT, bool PRE = false>
-__global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
+__global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_kernel(Params p) {
+  constexpr int NBP = PRE ? NBP_PRE : attn::NBP;
   using TL = Tile<D, KVT>;
-  using SM = PvSmem<D, RP, KVT>;
+  using SM = PvSmem<D, RP, KVT, NBP>;
   constexpr int ROWB = TL::ROWB, SWZ = TL::SWZ, TILEB = TL::TILEB;
   constexpr int CE = Chunk<KVT>::E;
   constexpr int KG = 512 / D;   // PV key groups
@@ -666,10 +673,16 @@ __global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
   const int kvh = blockIdx.y / p.head_slices, hslice = blockIdx.y % p.head_slices;
   const int req = blockIdx.z / p.qtiles, qtile = blockIdx.z % p.qtiles;
   int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
-  if (kr_hi < 0) return;  // uniform over the CTA
+  if (kr_hi < 0) {  // uniform over the CTA
+    if constexpr (PRE) wait_dependencies();  // the launch ends after the one it overlaps
+    return;
+  }
   if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
   const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
-  if (chunk > 0 && kb >= kr_hi) return;
+  if (chunk > 0 && kb >= kr_hi) {
+    if constexpr (PRE) wait_dependencies();
+    return;
+  }
   const int ke = min(kb + CHUNK, kr_hi);
   const int ntiles = (ke - kb + KT - 1) / KT;
   const int nk = ntiles * KT;
@@ -681,20 +694,25 @@ __global__ void __launch_bounds__(THREADS) chunk_pv_kernel(Params p) {
   const float scale = ldexpf(1.0f, p.frac);
   const float inv_scale = ldexpf(1.0f, -p.frac);
 
-  // the unit's scores (written by kernel 1) ride with the first V tile
-  {
+  TileCopier<D, KVT> cp(p, req, kb, ke, kvh);
+  // PRE: the scores and maxima are those of launches that may still run
+  auto load_scores = [&]() {
     const float* src = p.ws_s + unit * (RP * CHUNK);
     const int per_row = nk / 4;  // 16-byte pieces per row
     for (int e = t; e < RP * per_row; e += THREADS) {
       const int i = e / per_row, c = e % per_row;
       cp_async16(P_all + i * CHUNK + 4 * c, src + i * CHUNK + 4 * c, 16);
     }
-  }
-  TileCopier<D, KVT> cp(p, req, kb, ke, kvh);
+  };
+  if constexpr (!PRE) load_scores();  // they (written by kernel 1) ride with the first V tile
 #pragma unroll
   for (int s0 = 0; s0 < NBP - 1; ++s0) {
     if (s0 < ntiles)
       cp.issue(p.v, p.v_sb, p.v_ss, p.v_sh, s0, kvbuf + s0 * TILEB, cp.block_of(s0));
+    if (PRE && s0 == 0) {
+      wait_dependencies();
+      load_scores();
+    }
     cp_async_commit();
   }
   int next_blk = (NBP - 1 < ntiles) ? cp.block_of(NBP - 1) : -1;
@@ -1027,25 +1045,18 @@ static int pick_rp_chunked(const Params& p, int rp, int bits, int kv_dtype, int 
 
 template <int D, int RP, int BITS, typename KVT>
 static int launch_suffix_t(const Params& p, bool pv, int req, int ys, cudaStream_t st) {
-  constexpr bool rq = RP == 4;
   const dim3 grid((unsigned)p.nchunk_max, (unsigned)ys, (unsigned)((int64_t)req * p.qtiles));
   if (pv) {
     static bool done[64] = {false};
-    const size_t s2 = PvSmem<D, RP, KVT>::bytes;
+    const size_t s2 = PvSmem<D, RP, KVT, NBP_PRE>::bytes;
     auto k2 = chunk_pv_kernel<D, RP, BITS, KVT, true>;
     const int rc = configure((const void*)k2, s2, done);
     if (rc != FXPR_OK) return rc;
-    k2<<<grid, THREADS, s2, st>>>(p);
-    return check_launch("fxpr_shared_prefix_attention_fxp (pv)");
+    return launch_overlapped(k2, grid, s2, st, p, "fxpr_shared_prefix_attention_fxp (pv)");
   }
-  const size_t s1 = rq ? ScoreSmem<D, RP, KVT, KTC>::bytes : ScoreSmem<D, RP, KVT>::bytes;
+  const size_t s1 = ScoreSmem<D, RP, KVT>::bytes;
   const bool plain = !(p.softcap_log2 > 0.0f) && p.alibi == nullptr && p.window <= 0;
-  void (*k1)(Params);
-  if constexpr (rq) {
-    k1 = plain ? chunk_scores_rq_kernel<D, BITS, KVT, true, true> : chunk_scores_rq_kernel<D, BITS, KVT, false, true>;
-  } else {
-    k1 = plain ? chunk_scores_kernel<D, RP, BITS, KVT, true, true> : chunk_scores_kernel<D, RP, BITS, KVT, false, true>;
-  }
+  auto k1 = plain ? chunk_scores_kernel<D, RP, BITS, KVT, true, true> : chunk_scores_kernel<D, RP, BITS, KVT, false, true>;
   static bool done[2][64] = {{false}};
   const int rc = configure((const void*)k1, s1, done[plain ? 1 : 0]);
   if (rc != FXPR_OK) return rc;

@@ -148,6 +148,30 @@ template <typename T> __device__ __forceinline__ float absmax_value(uint32_t m) 
   }
 }
 
+// Launches that overlap the one before on their stream (programmatic dependent
+// launch): a kernel whose launch is `launch_overlapped` may start once every
+// CTA of the one before has called `launch_dependents` or left, and sees that
+// one's results (and, if it waited itself, those before) only after
+// `wait_dependencies`.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_dependencies() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename Arg>
+inline int launch_overlapped(void (*kernel)(Arg), dim3 grid, size_t smem, cudaStream_t st, const Arg& arg,
+                             const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, arg);
+  return check_launch(what);
+}
+
 // decode path for grouped-query batches (attention_decode.cu)
 bool decode_supported(const fxpr_attention_params* a, int G);
 int64_t decode_workspace_bytes(int items, int kmax, int D);

@@ -3,6 +3,9 @@
 // and converted once for a tile of rows of all requests instead of once per
 // request.
 //
+// Four launches behind a memset; each but the first may start while the one
+// before still runs, and waits for it before it reads its results.
+//
 //   clear    row maxima, normalisers and PV sums (one memset)
 //   scores   suffix: each request's own keys (chunk kernels, from key0 on)
 //            prefix: tiles of 16/32/64 rows x 64 keys
@@ -45,6 +48,8 @@ struct Args {
   int64_t units;    // kv heads * tiles * key_tiles, cut into equal slices over the CTAs
   float score_mul;  // scale_log2 * 2^-f (the scaling by 2^-f is exact: one rounding, as in two steps)
   int q_vec;        // q rows are 16-byte aligned
+  int page_even;    // keys 2i and 2i + 1 lie on one page
+  int later_pass;   // the scores' memory is still read by the pass before
 };
 
 // Rows of a tile: token, head, position and the range of keys [low, high) of
@@ -151,6 +156,8 @@ __global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(con
   const int krow = t / (DC / 8), kcol = (t % (DC / 8)) * 8;
   int64_t u0 = a.units * blockIdx.x / gridDim.x;
   const int64_t u1 = a.units * (blockIdx.x + 1) / gridDim.x;
+  launch_dependents();
+  if (a.later_pass) wait_dependencies();
 
   while (u0 < u1) {
     const int combo = (int)(u0 / a.key_tiles), kt0 = (int)(u0 % a.key_tiles);
@@ -331,6 +338,7 @@ __global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(con
       if (lane == 0 && rows.tok[r] >= 0) atomicMax(&p.row_max[(int64_t)rows.tok[r] * p.num_heads + rows.head[r]], m);
     }
   }
+  wait_dependencies();  // complete only after the suffix scores: who waits for this kernel has both
 }
 
 // ---------------------------------------------------------------------------
@@ -375,12 +383,18 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
   const double scale_d = ldexp(1.0, p.frac);
   const float vthr = __double2float_rd(fmin(65504.5, 4194304.0 / (scale_d * (1.0 + 1.0 / 1024))));
   const float2 C2 = make_float2(kMagic, kMagic), ONE2 = make_float2(p.one, p.one);
+  const bool small_frac = p.frac <= 22;  // p * 2^f <= 2^22: the magic constant rounds it
+  // bf16 -> fp16 is exact from 2^-17 up to 65504, and below |p * v * 2^f| < 1/2 either way when f <= 16; beyond 65504
+  // (infinite in fp16) the tile is not fast and its V is converted again
+  const bool v_exact16 = std::is_same<T, __half>::value || p.frac <= 16;
   const int prow = t / TPR;             // p phase: this row, keys 4 * (t % TPR) + 4 * TPR * u
   const int dl = t % LD, grp = t / LD;  // this thread's dims 4 * dl.., rows grp * TM..
   const int vc = dl / 2, vj = (dl & 1) * 2, vx = (vc >> 1) & 3;
   const int v0 = (vc * 4 + (vj ^ vx)) * 16, v1 = (vc * 4 + ((vj + 1) ^ vx)) * 16;
   int64_t u0 = a.units * blockIdx.x / gridDim.x;
   const int64_t u1 = a.units * (blockIdx.x + 1) / gridDim.x;
+  bool waited = false;
+  launch_dependents();
 
   while (u0 < u1) {
     const int combo = (int)(u0 / a.key_tiles), kt0 = (int)(u0 % a.key_tiles);
@@ -391,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
     tile_rows<RT>(a, a.tile0 + tile, kvh, rows);
     const bool live = rows.tok[prow] >= 0;
     const int64_t row_id = live ? (int64_t)rows.tok[prow] * p.num_heads + rows.head[prow] : 0;
-    const float m = live ? from_ordered(p.row_max[row_id]) : 0.0f;
+    float m = 0.0f;
     const float* src = a.scores + (((int64_t)kvh * a.tiles + tile) * RT + prow) * p.key0 + kt0 * KT64 + 4 * (t % TPR);
     UAcc den = 0;
 
@@ -404,14 +418,21 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
         at_a[u] = at_b[u] = -1;
         if (ti >= n) continue;
         const int unit = t + u * THREADS, j = (kt0 + ti) * KT64 + 2 * (unit / (D / 8)), d = (unit % (D / 8)) * 8;
-        const int ba = block_of(a, j), bb = block_of(a, j + 1);
+        const int ba = block_of(a, j);
         if (ba >= 0) at_a[u] = key_offset(p, j, ba, p.v_sb, p.v_ss, p.v_sh, kvh) + d;
-        if (bb >= 0) at_b[u] = key_offset(p, j + 1, bb, p.v_sb, p.v_ss, p.v_sh, kvh) + d;
+        if (a.page_even) {
+          if (ba >= 0) at_b[u] = at_a[u] + p.v_ss;
+        } else {
+          const int bb = block_of(a, j + 1);
+          if (bb >= 0) at_b[u] = key_offset(p, j + 1, bb, p.v_sb, p.v_ss, p.v_sh, kvh) + d;
+        }
       }
     };
-    auto load = [&](int ti) {
+    auto load_scores = [&](int ti) {
 #pragma unroll
       for (int u = 0; u < SV; ++u) sc[u] = *reinterpret_cast<const float4*>(src + ti * KT64 + 4 * TPR * u);
+    };
+    auto load_v = [&](int ti) {
 #pragma unroll
       for (int u = 0; u < VU; ++u) {
         va[u] = vb[u] = make_uint4(0, 0, 0, 0);
@@ -428,12 +449,15 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = -0.0f;  // a masked key: no contribution, whatever its V holds
-          if (live && s[e] != -INFINITY) {
-            x = prim_exp2(__fsub_rn(s[e], m));
-            den += (UAcc)f2x_f32<BITS>(x, scale);
-          }
+          // a masked key (-inf, as every key of a row that is none) is -0: no
+          // contribution, whatever its V holds
+          const float x = s[e] == -INFINITY ? -0.0f : prim_exp2(__fsub_rn(s[e], m));
           v[e] = __fmul_rn(x, scale);
+          if (small_frac) {
+            den += (UAcc)(__float_as_uint(__fadd_rn(v[e], kMagic)) - (uint32_t)kMagicBits);
+          } else {
+            den += (UAcc)f2x_scaled<BITS>(v[e]);
+          }
         }
         *reinterpret_cast<float4*>(pd + 4 * TPR * u) = make_float4(v[0], v[1], v[2], v[3]);
       }
@@ -462,16 +486,21 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][e] = 0u;
-    auto flush = [&]() {
+    auto flush = [&](int fast_tiles) {
+      const uint32_t bias = (uint32_t)fast_tiles * (uint32_t)KT64 * (uint32_t)kMagicBits;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int r = grp * TM + i;
-        if (rows.tok[r] < 0) continue;
+        if (rows.tok[r] < 0) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][e] = 0u;
+          continue;
+        }
         unsigned long long* dst = p.row_acc + ((int64_t)rows.tok[r] * p.num_heads + rows.head[r]) * D + 4 * dl;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const unsigned long long v =
-              BITS == 64 ? (unsigned long long)(long long)(int32_t)acc[i][e] : (unsigned long long)acc[i][e];
+          const uint32_t s = acc[i][e] - bias;
+          const unsigned long long v = BITS == 64 ? (unsigned long long)(long long)(int32_t)s : (unsigned long long)s;
           if (v) atomicAdd(dst + e, v);
           acc[i][e] = 0u;
         }
@@ -479,10 +508,18 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
     };
 
     addresses(0);
-    load(0);
+    load_v(0);
+    if (!waited) wait_dependencies();  // the scores and maxima are those of launches that may still run
+    waited = true;
+    load_scores(0);
+    if (live) m = from_ordered(p.row_max[row_id]);
     store(0);
-    if (n > 1) load(1);
+    if (n > 1) {
+      load_scores(1);
+      load_v(1);
+    }
     __syncthreads();
+    int fast_tiles = 0;
     for (int ti = 0; ti < n; ++ti) {
       const bool fast = __uint_as_float(v_max[ti % 3]) < vthr;  // uniform over the CTA
       if (t == 0) v_max[(ti + 2) % 3] = 0u;
@@ -512,10 +549,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
               }
           }
         }
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][e] -= (uint32_t)KT64 * (uint32_t)kMagicBits;
+        ++fast_tiles;
       } else {  // values the constant cannot round: the definition's clamp and convert
 #pragma unroll 1
         for (int i = 0; i < TM; ++i) {
@@ -528,18 +562,24 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
               const float ps = pb[i * P_LD + k];
               if (__float_as_uint(ps) == 0x80000000u) continue;
               const float vv = reinterpret_cast<const float*>(vs + (size_t)(k / 2) * D * 8 + (e < 2 ? v0 : v1))[2 * (e & 1) + (k & 1)];
-              s += (UAcc)f2x_scaled<BITS>(__fmul_rn(ps, vv));
+              s += (UAcc)f2x_scaled<BITS>(__fmul_rn(ps, __half2float(__float2half_rn(vv))));
             }
             if (s) atomicAdd(p.row_acc + ((int64_t)rows.tok[r] * p.num_heads + rows.head[r]) * D + 4 * dl + e, (unsigned long long)s);
           }
         }
       }
-      if (BITS == 64 && (ti + 1) % RUN == 0) flush();
+      if (BITS == 64 && (ti + 1) % RUN == 0) {
+        flush(fast_tiles);
+        fast_tiles = 0;
+      }
       if (ti + 1 < n) store(ti + 1);
-      if (ti + 2 < n) load(ti + 2);
+      if (ti + 2 < n) {
+        load_scores(ti + 2);
+        load_v(ti + 2);
+      }
       __syncthreads();
     }
-    flush();
+    flush(fast_tiles);
 #pragma unroll
     for (int o = 1; o < TPR; o <<= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
     if (t % TPR == 0 && live && den) atomicAdd(p.row_den + row_id, (unsigned long long)den);
@@ -573,15 +613,13 @@ static int launch(Args& a, bool pv, int kv_heads, cudaStream_t st) {
     auto k = prefix_pv_kernel<D, RT, BITS, T>;
     const int rc = configure((const void*)k, PvSmem<D, RT>::bytes, done);
     if (rc != FXPR_OK) return rc;
-    k<<<grid, THREADS, PvSmem<D, RT>::bytes, st>>>(a);
-    return check_launch("fxpr_shared_prefix_attention_fxp (prefix pv)");
+    return launch_overlapped(k, dim3(grid), PvSmem<D, RT>::bytes, st, a, "fxpr_shared_prefix_attention_fxp (prefix pv)");
   }
   static bool done[2][64] = {{false}};
   auto k = plain ? prefix_scores_kernel<D, RT, BITS, T, true> : prefix_scores_kernel<D, RT, BITS, T, false>;
   const int rc = configure((const void*)k, ScoresSmem<D, RT>::bytes, done[plain ? 1 : 0]);
   if (rc != FXPR_OK) return rc;
-  k<<<grid, THREADS, ScoresSmem<D, RT>::bytes, st>>>(a);
-  return check_launch("fxpr_shared_prefix_attention_fxp (prefix scores)");
+  return launch_overlapped(k, dim3(grid), ScoresSmem<D, RT>::bytes, st, a, "fxpr_shared_prefix_attention_fxp (prefix scores)");
 }
 
 template <int D, int RT>
@@ -612,6 +650,8 @@ int launch_prefix(const Params& p, bool pv, int D, int row_tile, int bits, int k
   a.tile0 = tile0;
   a.tiles = tiles;
   a.score_mul = ldexpf(p.scale_log2, -p.frac);
+  a.page_even = p.page % 2 == 0;
+  a.later_pass = tile0 > 0;
   a.q_vec = (uintptr_t)p.q % 16 == 0 && p.q_st % 8 == 0 && p.q_sh % 8 == 0;
   if (D == 64) return prefix::pick_rows<64>(a, pv, row_tile, bits, kv_dtype, p.num_kv_heads, st);
   return prefix::pick_rows<128>(a, pv, row_tile, bits, kv_dtype, p.num_kv_heads, st);

@@ -274,9 +274,9 @@ def test_batch_invariance_and_repeat():
 
 @pytest.mark.gpu
 def test_many_rows_in_passes():
-    """More row tiles than the scores' workspace holds (64 MB): the prefix runs in passes."""
+    """More row tiles than the scores' workspace holds (128 MB): the prefix runs in passes."""
     prefix = 2048
-    b = _batch([96] * 16, [100] * 16, prefix, 8, 1, 64, seed=16)
+    b = _batch([96] * 24, [100] * 24, prefix, 8, 1, 64, seed=16)
     _same(b, prefix, o_dtype=BF)
 
 

@@ -768,14 +768,16 @@ int check_alignment(const fxpr_attention_params* a) {
 // ---------------------------------------------------------------------------
 // shared prefix: which calls take the prefix kernels, and their workspace
 // ---------------------------------------------------------------------------
-#ifndef FXPR_PREFIX_MIN_ROWS
-#define FXPR_PREFIX_MIN_ROWS 1
-#endif
-#ifndef FXPR_PREFIX_MIN_KEYS
-#define FXPR_PREFIX_MIN_KEYS 64
-#endif
-constexpr int kPrefixMinRows = FXPR_PREFIX_MIN_ROWS;
-constexpr int kPrefixMinKeys = FXPR_PREFIX_MIN_KEYS;
+// Device time of the unified attention over the prefix kernels' (graph
+// replays, 16-bit, 32 query heads unless said):
+//   where it runs its chunk kernels (several queries a request, groups other
+//   than 4, odd pages): prefix of 128 keys 0.6 to 1.35, 512 keys 1.1 to 3.0,
+//   2048 keys 1.4 to 5.7; taken from 256 keys on;
+//   where it runs its decode kernels, (row, key) pairs of the prefix 1 M: 0.9
+//   to 1.05, 4 M: 1.08 (head_dim 128) and 1.27 (64), 8 M: 1.2; fewer launches
+//   make it the faster one for small batches. Taken from 2 M pairs on.
+constexpr int kPrefixMinKeys = 256;
+constexpr int64_t kPrefixMinDecodePairs = 2ll << 20;
 constexpr int64_t kPrefixScores = 128ll << 20;  // about the L2
 
 struct PrefixPlan {
@@ -794,8 +796,11 @@ PrefixPlan prefix_plan_of(const fxpr_attention_params* a, int prefix_len, int64_
   key0 = key0 / attn::KT * attn::KT;  // the last keys of a ragged prefix run with each request's own
   const int64_t rows_kv = tokens * pl.G;
   if ((a->head_dim != 64 && a->head_dim != 128) || !half(a->q_dtype) || !half(a->kv_dtype) ||
-      key0 < kPrefixMinKeys || rows_kv < kPrefixMinRows || a->num_blocks <= 0)
+      key0 < kPrefixMinKeys || a->num_blocks <= 0 ||
+      (pl.decode_kmax > 0 && rows_kv * a->num_kv_heads * key0 < kPrefixMinDecodePairs))
     return pp;
+  auto fits = [](int64_t s) { return s >= 0 && s <= 0x7fffffffLL; };
+  if (!fits(a->k_stride_blk) || !fits(a->k_stride_slot) || !fits(a->v_stride_blk) || !fits(a->v_stride_slot)) return pp;
   pp.key0 = key0;
   pp.row_tile = rows_kv <= 16 ? 16 : rows_kv <= 32 ? 32 : 64;
   const int64_t tiles = cdiv(rows_kv, pp.row_tile);

@@ -49,6 +49,7 @@ struct Args {
   float score_mul;  // scale_log2 * 2^-f (the scaling by 2^-f is exact: one rounding, as in two steps)
   int q_vec;        // q rows are 16-byte aligned
   int page_even;    // keys 2i and 2i + 1 lie on one page
+  int k_sb, k_ss, v_sb, v_ss;  // cache strides of a block and a key (elements; the host checks that they fit)
   int later_pass;   // the scores' memory is still read by the pass before
 };
 
@@ -59,6 +60,7 @@ struct Args {
 template <int RT>
 struct Rows {
   int tok[RT], head[RT], pos[RT], low[RT], high[RT];
+  int all_low, all_high;  // keys that every row of the batch in the tile sees
 };
 template <int RT>
 __device__ __forceinline__ void tile_rows(const Args& a, int tile, int kvh, Rows<RT>& rows) {
@@ -68,6 +70,10 @@ __device__ __forceinline__ void tile_rows(const Args& a, int tile, int kvh, Rows
   if (t < RT) {
     rows.tok[t] = -1;
     rows.head[t] = rows.pos[t] = rows.low[t] = rows.high[t] = 0;
+  }
+  if (t == 0) {
+    rows.all_low = 0;
+    rows.all_high = p.key0;
   }
   __syncthreads();
   const int row0 = tile * RT, row1 = min(row0 + RT, a.tokens * p.group);
@@ -81,18 +87,31 @@ __device__ __forceinline__ void tile_rows(const Args& a, int tile, int kvh, Rows
       // the reference walks keys to the end of its 64-row query block
       int high = p.causal ? min(seq, ctx + (off / 64 + 1) * 64) : seq;
       if (p.causal) high = min(high, pos + 1);
+      high = min(high, p.key0);
+      const int low = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+      if (high < p.key0) atomicMin(&rows.all_high, high);
+      if (low > 0) atomicMax(&rows.all_low, low);
       for (int g = 0; g < p.group; ++g) {
         const int i = tok * p.group + g - row0;
         if (i < 0 || i >= RT) continue;
         rows.tok[i] = tok;
         rows.head[i] = kvh * p.group + g;
         rows.pos[i] = pos;
-        rows.low[i] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-        rows.high[i] = min(high, p.key0);
+        rows.low[i] = low;
+        rows.high[i] = high;
       }
     }
   }
   __syncthreads();
+}
+
+// The base-2 exponential of the unified attention with subnormal results
+// flushed to zero: those round to 0 on the grid, and so do their products with
+// any finite V.
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 template <typename T> __device__ __forceinline__ float2 pair_of(uint32_t w) {
@@ -103,10 +122,10 @@ template <typename T> __device__ __forceinline__ float2 pair_of(uint32_t w) {
   }
 }
 
-__device__ __forceinline__ int64_t key_offset(const Params& p, int j, int blk, int64_t sb, int64_t ss, int64_t sh,
-                                              int kvh) {
+// element offset of key j, on block blk, from its KV head's first key
+__device__ __forceinline__ int64_t key_offset(const Params& p, int j, int blk, int sb, int ss) {
   const int slot = p.page_shift >= 0 ? (j & (p.page - 1)) : j % p.page;
-  return (int64_t)blk * sb + (int64_t)slot * ss + (int64_t)kvh * sh;
+  return (int64_t)blk * sb + (int64_t)slot * ss;
 }
 // physical block of key j of the first request (whose prefix pages are
 // everyone's); -1, which reads zeros, for an id outside the cache
@@ -128,16 +147,16 @@ struct ScoresSmem {
   static constexpr size_t off_k = (size_t)RT * Q_LD * 4;
   static constexpr size_t bytes = off_k + 2ull * KT64 * K_LD * 4;
 };
-#ifndef FXPR_PRE_SU
-#define FXPR_PRE_SU 4
-#endif
-constexpr int SU = FXPR_PRE_SU;
-#ifndef FXPR_PRE_SB
-#define FXPR_PRE_SB 3
-#endif
+// 2 CTAs per SM and 4 k-steps unrolled: 64 requests behind 4096 keys, 32 / 8
+// heads x 128, bf16 (1.07 G products): 84.4 us, 12.7 T products/s of the 18.4
+// that this tile's inner loop alone reaches; 3 CTAs 88.4 us (the 2048 units do
+// not divide as well), 16 k-steps 83.2 us here but 109.5 against 106.7 us with
+// head_dim 64.
+constexpr int SCORES_CTAS = 2;
+constexpr int SU = 4;
 
 template <int D, int RT, int BITS, typename T, bool PL>
-__global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(const __grid_constant__ Args a) {
   constexpr int TM = RT / 8, TN = KT64 / 32, NCH = D / DC;
   constexpr int Q_LD = ScoresSmem<D, RT>::Q_LD;
   constexpr int LOADS = KT64 * DC / 8 / THREADS;  // 16-byte loads of K per thread and step
@@ -149,7 +168,6 @@ __global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(con
   __shared__ uint32_t q_max, k_max[3];
 
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const T* kbase = reinterpret_cast<const T*>(p.k);
   const float scale = ldexpf(1.0f, p.frac);
   const float2 C2 = make_float2(kMagic, kMagic);
   // K staging: thread t moves 8 dims of key rows t / 8 + 32 * u of a tile
@@ -201,6 +219,7 @@ __global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(con
       if (lane == 0) atomicMax(&q_max, qo);
     }
 
+    const T* khead = reinterpret_cast<const T*>(p.k) + kvh * p.k_sh;
     const int steps = n * NCH;
     int64_t at[LOADS], at_next[LOADS];  // element offsets of this thread's key rows; -1 outside the cache
     auto addresses = [&](int ti, int64_t (&x)[LOADS]) {
@@ -209,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(con
         x[u] = -1;
         if (ti >= n) continue;
         const int j = (kt0 + ti) * KT64 + krow + (THREADS / (DC / 8)) * u, blk = block_of(a, j);
-        if (blk >= 0) x[u] = key_offset(p, j, blk, p.k_sb, p.k_ss, p.k_sh, kvh) + kcol;
+        if (blk >= 0) x[u] = key_offset(p, j, blk, a.k_sb, a.k_ss);
       }
     };
     uint4 raw[LOADS];
@@ -223,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(con
 #pragma unroll
       for (int u = 0; u < LOADS; ++u) {
         raw[u] = make_uint4(0, 0, 0, 0);
-        if (at[u] >= 0) raw[u] = *reinterpret_cast<const uint4*>(kbase + at[u] + ch * DC);
+        if (at[u] >= 0) raw[u] = *reinterpret_cast<const uint4*>(khead + kcol + at[u] + ch * DC);
       }
     };
     auto store = [&](int it) {
@@ -297,7 +316,7 @@ __global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(con
             const int kblk = block_of(a, key);
             typename std::conditional<BITS == 64, unsigned long long, uint32_t>::type s = 0;
             if (rows.tok[r] >= 0 && kblk >= 0) {
-              const T* kr = kbase + key_offset(p, key, kblk, p.k_sb, p.k_ss, p.k_sh, kvh);
+              const T* kr = khead + key_offset(p, key, kblk, a.k_sb, a.k_ss);
               const int64_t qo = (int64_t)rows.tok[r] * p.q_st + (int64_t)rows.head[r] * p.q_sh;
               for (int d = 0; d < D; ++d)
                 s += (decltype(s))f2x_f32<BITS>(__fmul_rn(load_f32(p.q, p.q_dtype, qo + d), to_f32(kr[d])), scale);
@@ -310,20 +329,36 @@ __global__ void __launch_bounds__(THREADS, FXPR_PRE_SB) prefix_scores_kernel(con
                 if (e == i * TN + j) acc[i][j] = __float_as_uint(f);  // kept as its fp32 value
           }
         }
+        float* dst = out + ti * KT64;
+        const int key0 = (kt0 + ti) * KT64;
+        if (PL && fast && key0 >= rows.all_low && key0 + KT64 <= rows.all_high) {  // the usual tile: every row sees every key
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const int r = warp * TM + i, low = rows.low[r], high = rows.high[r];
+          for (int i = 0; i < TM; ++i) {
 #pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            const int key = (kt0 + ti) * KT64 + lane + 32 * j;
-            float qk = __fmul_rn(fast ? __int2float_rn((int32_t)acc[i][j]) : __uint_as_float(acc[i][j]), a.score_mul);
-            if constexpr (!PL) {
-              if (p.softcap_log2 > 0.0f) qk = __fmul_rn(p.softcap_log2, prim_tanh(__fmul_rn(qk, p.softcap_rcp)));
-              if (p.alibi) qk = __fmaf_rn(p.alibi[rows.head[r]], __fsub_rn((float)key, (float)rows.pos[r]), qk);
+            for (int j = 0; j < TN; ++j) {
+              const float s = __fmul_rn(__int2float_rn((int32_t)acc[i][j]), a.score_mul);
+              dst[32 * j] = s;
+              rmax[i] = fmaxf(rmax[i], s);
             }
-            const float s = key >= low && key < high ? qk : -INFINITY;
-            out[(int64_t)i * p.key0 + ti * KT64 + 32 * j] = s;
-            rmax[i] = fmaxf(rmax[i], s);
+            dst += p.key0;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            const int r = warp * TM + i, low = rows.low[r], high = rows.high[r];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+              const int key = key0 + lane + 32 * j;
+              float qk = __fmul_rn(fast ? __int2float_rn((int32_t)acc[i][j]) : __uint_as_float(acc[i][j]), a.score_mul);
+              if constexpr (!PL) {
+                if (p.softcap_log2 > 0.0f) qk = __fmul_rn(p.softcap_log2, prim_tanh(__fmul_rn(qk, p.softcap_rcp)));
+                if (p.alibi) qk = __fmaf_rn(p.alibi[rows.head[r]], __fsub_rn((float)key, (float)rows.pos[r]), qk);
+              }
+              const float s = key >= low && key < high ? qk : -INFINITY;
+              dst[32 * j] = s;
+              rmax[i] = fmaxf(rmax[i], s);
+            }
+            dst += p.key0;
           }
         }
       }
@@ -355,10 +390,9 @@ struct PvSmem {
   static constexpr size_t off_p = 2 * v_buf;
   static constexpr size_t bytes = off_p + 2 * p_buf;
 };
-#ifndef FXPR_PRE_VU
-#define FXPR_PRE_VU 4
-#endif
-constexpr int VU_UNROLL = FXPR_PRE_VU;
+// At the sizes above 122.4 us, 8.8 T products/s of the 12.5 of the inner loop
+// alone; 16 k-steps unrolled 132 us.
+constexpr int VU_UNROLL = 4;
 
 template <int D, int RT, int BITS, typename T>
 __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_constant__ Args a) {
@@ -378,7 +412,6 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
 
   const int t = threadIdx.x, lane = t & 31;
   const float scale = ldexpf(1.0f, p.frac);
-  const T* vbase = reinterpret_cast<const T*>(p.v);
   // max|v| <= 65504 (finite after the cast) and max|v| * (1 + 2^-10) * 2^f < 2^22, with p <= 1
   const double scale_d = ldexp(1.0, p.frac);
   const float vthr = __double2float_rd(fmin(65504.5, 4194304.0 / (scale_d * (1.0 + 1.0 / 1024))));
@@ -409,6 +442,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
     const float* src = a.scores + (((int64_t)kvh * a.tiles + tile) * RT + prow) * p.key0 + kt0 * KT64 + 4 * (t % TPR);
     UAcc den = 0;
 
+    const T* vhead = reinterpret_cast<const T*>(p.v) + kvh * p.v_sh;
     float4 sc[SV];
     uint4 va[VU], vb[VU];
     int64_t at_a[VU], at_b[VU];  // element offsets of the next tile's key pairs; -1 outside the cache
@@ -419,12 +453,12 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
         if (ti >= n) continue;
         const int unit = t + u * THREADS, j = (kt0 + ti) * KT64 + 2 * (unit / (D / 8)), d = (unit % (D / 8)) * 8;
         const int ba = block_of(a, j);
-        if (ba >= 0) at_a[u] = key_offset(p, j, ba, p.v_sb, p.v_ss, p.v_sh, kvh) + d;
+        if (ba >= 0) at_a[u] = key_offset(p, j, ba, a.v_sb, a.v_ss) + d;
         if (a.page_even) {
-          if (ba >= 0) at_b[u] = at_a[u] + p.v_ss;
+          if (ba >= 0) at_b[u] = at_a[u] + a.v_ss;
         } else {
           const int bb = block_of(a, j + 1);
-          if (bb >= 0) at_b[u] = key_offset(p, j + 1, bb, p.v_sb, p.v_ss, p.v_sh, kvh) + d;
+          if (bb >= 0) at_b[u] = key_offset(p, j + 1, bb, a.v_sb, a.v_ss) + d;
         }
       }
     };
@@ -436,8 +470,8 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
 #pragma unroll
       for (int u = 0; u < VU; ++u) {
         va[u] = vb[u] = make_uint4(0, 0, 0, 0);
-        if (at_a[u] >= 0) va[u] = *reinterpret_cast<const uint4*>(vbase + at_a[u]);
-        if (at_b[u] >= 0) vb[u] = *reinterpret_cast<const uint4*>(vbase + at_b[u]);
+        if (at_a[u] >= 0) va[u] = *reinterpret_cast<const uint4*>(vhead + at_a[u]);
+        if (at_b[u] >= 0) vb[u] = *reinterpret_cast<const uint4*>(vhead + at_b[u]);
       }
       addresses(ti + 1);
     };
@@ -449,9 +483,8 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          // a masked key (-inf, as every key of a row that is none) is -0: no
-          // contribution, whatever its V holds
-          const float x = s[e] == -INFINITY ? -0.0f : prim_exp2(__fsub_rn(s[e], m));
+          // a masked key (-inf) is -0: no contribution, whatever its V holds
+          const float x = s[e] == -INFINITY ? -0.0f : exp2_ftz(__fsub_rn(s[e], m));
           v[e] = __fmul_rn(x, scale);
           if (small_frac) {
             den += (UAcc)(__float_as_uint(__fadd_rn(v[e], kMagic)) - (uint32_t)kMagicBits);
@@ -606,7 +639,7 @@ static int launch(Args& a, bool pv, int kv_heads, cudaStream_t st) {
   const bool plain = !(a.p.softcap_log2 > 0.0f) && a.p.alibi == nullptr && a.p.window <= 0;
   a.key_tiles = a.p.key0 / KT64;
   a.units = (int64_t)kv_heads * a.tiles * a.key_tiles;
-  const int64_t resident = (int64_t)num_sms() * (pv ? 2 : FXPR_PRE_SB);
+  const int64_t resident = (int64_t)num_sms() * (pv ? 2 : SCORES_CTAS);
   const unsigned grid = (unsigned)(a.units < resident ? a.units : resident);
   if (pv) {
     static bool done[64] = {false};
@@ -650,6 +683,10 @@ int launch_prefix(const Params& p, bool pv, int D, int row_tile, int bits, int k
   a.tile0 = tile0;
   a.tiles = tiles;
   a.score_mul = ldexpf(p.scale_log2, -p.frac);
+  a.k_sb = (int)p.k_sb;
+  a.k_ss = (int)p.k_ss;
+  a.v_sb = (int)p.v_sb;
+  a.v_ss = (int)p.v_ss;
   a.page_even = p.page % 2 == 0;
   a.later_pass = tile0 > 0;
   a.q_vec = (uintptr_t)p.q % 16 == 0 && p.q_st % 8 == 0 && p.q_sh % 8 == 0;

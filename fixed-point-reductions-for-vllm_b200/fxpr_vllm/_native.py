@@ -196,7 +196,8 @@ def on_device(device: torch.device):
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)  # without a Stream object around it
 
 
 def dcode(t: torch.Tensor) -> int:

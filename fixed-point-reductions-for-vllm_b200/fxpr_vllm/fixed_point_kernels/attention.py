@@ -157,10 +157,10 @@ def shared_prefix_attention_fxp(
 
     The first ``common_prefix_len // page`` entries of every block-table row
     are the same pages (those of row 0 are read), and the keys of a last page
-    that the prefix covers in part are equal in every request's own page. The
-    result has the bits of ``unified_attention_fxp``, except that a masked key
-    contributes nothing even where its V is infinite or NaN and that a row
-    which sees no key is 0. Rows of ``o`` behind ``query_start_loc[-1]`` are
+    that the prefix covers in part are equal in every request's own page. With
+    finite V the result has the bits of ``unified_attention_fxp``; a masked key
+    contributes nothing even where its V is infinite or NaN, and a row which
+    sees no key is 0. Rows of ``o`` behind ``query_start_loc[-1]`` are
     left as they are. ``max_seq_len`` bounds every ``seq_lens`` entry when
     given, as there. Scratch is a tensor of the call, so calls on several
     streams and captured graphs share nothing."""

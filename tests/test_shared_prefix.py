@@ -106,13 +106,16 @@ def test_abi_refuses_and_sizes_its_workspace():
 @pytest.mark.parametrize("bits", [32, 64])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("qlens, suffix, prefix, H, KVH, page", [
-    ([1] * 5, [1, 17, 200, 513, 1100], 256, 8, 2, 16),       # decode, own keys over several chunks
-    ([1] * 9, [1] * 9, 64, 4, 1, 16),                        # one tile of keys, nothing but the query behind it
-    ([1] * 40, list(range(1, 41)), 1000, 8, 2, 16),          # ragged prefix (last page copied), several row tiles
+    ([1] * 5, [1, 17, 200, 513, 1100], 256, 8, 4, 16),       # decode, own keys over several chunks
+    ([1] * 9, [1] * 9, 256, 4, 4, 16),                       # no group, nothing but the query behind the prefix
+    ([1] * 40, list(range(1, 41)), 1000, 16, 2, 16),         # ragged prefix (last page copied), several row tiles
+    ([1] * 40, [3] * 40, 260, 12, 4, 16),                    # rows of a token on two tiles
+    ([1] * 32, list(range(1, 33)), 4096, 16, 4, 16),         # groups of 4 with enough of a prefix
+    ([1] * 6, list(range(1, 7)), 512, 8, 2, 16),             # and without: the unified decode kernels
     ([5, 1, 3, 9, 2], [5, 8, 3, 30, 2], 333, 8, 4, 8),       # verification, group of 2, small pages
     ([70, 1, 130], [70, 1, 200], 704, 7, 1, 48),             # chunked prefill, group of 7, pages across tiles
     ([1], [3], 500, 16, 2, 16),                              # one request
-    ([2, 0, 3, 0], [2, 0, 9, 5], 128, 2, 2, 1),              # requests without queries, pages of one key
+    ([2, 0, 3, 0], [2, 0, 9, 5], 290, 2, 2, 1),              # requests without queries, pages of one key
 ])
 def test_bits_of_the_unified_attention(qlens, suffix, prefix, H, KVH, page, D, bits):
     for dtype in (BF, HF):
@@ -130,7 +133,7 @@ def test_masks_and_scores(kw, qlens, suffix):
     if kw.pop("alibi", False):
         kw["alibi_slopes"] = (2.0 ** -torch.arange(1.0, 9.0) * LOG2E).cuda()
     for D, bits in ((64, 32), (128, 64)):
-        a = _same(_batch(qlens, suffix, 640, 8, 2, D, seed=3), 640, bits=bits, **kw)
+        a = _same(_batch(qlens, suffix, 640, 8, 4, D, seed=3), 640, bits=bits, **kw)
         assert a.isfinite().all()
 
 
@@ -176,7 +179,7 @@ def test_masked_places_do_not_count():
 @pytest.mark.gpu
 def test_short_and_padded_requests():
     """Requests shorter than the prefix, without keys or queries, and rows behind the last sequence."""
-    (q, kv, qsl, sl, bt), mq, ms = _batch([1] * 20, [5] * 20, 256, 8, 2, 128, seed=8, pad=11)
+    (q, kv, qsl, sl, bt), mq, ms = _batch([1] * 20, [5] * 20, 256, 8, 4, 128, seed=8, pad=11)
     sl[3], sl[4], sl[5] = 100, 1, 64
     _same(((q, kv, qsl, sl, bt), mq, ms), 256)
     sl[6] = 0  # a request that sees nothing: 0, where the unified attention has no defined value
@@ -241,7 +244,7 @@ def test_strides_types_and_other_forms():
 
 @pytest.mark.gpu
 def test_block_ids_outside_the_cache_read_zeros():
-    (q, kv, qsl, sl, bt), mq, ms = _batch([1] * 20, [5] * 20, 256, 8, 2, 128, seed=14)
+    (q, kv, qsl, sl, bt), mq, ms = _batch([1] * 20, [5] * 20, 256, 8, 4, 128, seed=14)
     bad = bt.clone()
     bad[0, 3], bad[0, 7] = kv.shape[0], -5
     a = torch.zeros(q.shape, device="cuda")
@@ -283,7 +286,7 @@ def test_many_rows_in_passes():
 @pytest.mark.gpu
 def test_streams_and_two_captured_graphs():
     """Two captured graphs replayed at the same time on two streams, and an eager call beside them, share no scratch."""
-    bs = [_batch([1] * 24, [9] * 24, 512, 8, 2, 128, seed=s) for s in (17, 18)]
+    bs = [_batch([1] * 24, [9] * 24, 512, 8, 4, 128, seed=s) for s in (17, 18)]
     want = [_same(b, 512) for b in bs]
     outs, graphs = [torch.zeros_like(w) for w in want], []
     for b, o in zip(bs, outs):

@@ -7,6 +7,13 @@ seq_lens, block_table, max_query_len, max_seq_len); the paged KV cache layout
 (``reshape_and_cache_flash``) are vLLM's. The attention itself is
 ``unified_attention_fxp`` on the B200 kernel, split over
 ``VLLM_FXP_NUM_KV_SPLITS`` KV splits (results do not depend on the count).
+
+Two additions to the reference's backend. When the engine's cascade attention
+is on (``disable_cascade_attn=False``) and all requests of a step share a
+prefix, ``shared_prefix_attention_fxp`` runs instead, with the same bits. With
+``VLLM_FXP_FUSED_ROPE=1`` the backend takes vLLM's fused rotary and cache
+update: the rotation then has one fixed arithmetic in every mode of the engine,
+where vLLM's own kernel and torch.compile's code round differently.
 """
 
 from __future__ import annotations
@@ -15,13 +22,36 @@ import logging
 
 import torch
 from vllm.v1.attention.backend import AttentionImpl, AttentionLayer, AttentionType
-from vllm.v1.attention.backends.triton_attn import TritonAttentionBackend
+from vllm.v1.attention.backends.triton_attn import TritonAttentionBackend, TritonAttentionMetadataBuilder
 
-from ..fixed_point_kernels.attention import unified_attention_fxp
+from ..fixed_point_kernels.attention import shared_prefix_attention_fxp, unified_attention_fxp
 from ..fixed_point_kernels.fixed_point import RCP_LN2
+from ..fixed_point_kernels.rope import rope_append_kv_fxp
 from .config import get_runtime_config
 
 logger = logging.getLogger("fxpr_vllm")
+
+
+class DeterministicAttentionMetadataBuilder(TritonAttentionMetadataBuilder):
+    """The Triton backend's metadata, with cascade attention from a common
+    prefix of ``MIN_PREFIX`` keys on (below, the shared-prefix operator runs
+    the unified kernels anyway)."""
+
+    MIN_PREFIX = 256
+
+    def use_cascade_attention(self, common_prefix_len: int, query_lens, num_query_heads: int,
+                              num_kv_heads: int, use_alibi: bool, use_sliding_window: bool,
+                              use_local_attention: bool, num_sms: int, dcp_world_size: int) -> bool:
+        return (common_prefix_len >= self.MIN_PREFIX and len(query_lens) > 1
+                and not use_local_attention and dcp_world_size <= 1)
+
+    def build(self, common_prefix_len: int, common_attn_metadata, fast_build: bool = False):
+        # the Triton builder's own cascade fields are not used (it leaves some
+        # of them unset): built without a prefix, which is then noted
+        metadata = super().build(0, common_attn_metadata, fast_build)
+        if common_prefix_len > 0:
+            metadata.use_cascade, metadata.common_prefix_len = True, common_prefix_len
+        return metadata
 
 
 class DeterministicAttentionBackend(TritonAttentionBackend):
@@ -37,6 +67,10 @@ class DeterministicAttentionBackend(TritonAttentionBackend):
     @staticmethod
     def get_impl_cls() -> type["DeterministicAttentionImpl"]:
         return DeterministicAttentionImpl
+
+    @staticmethod
+    def get_builder_cls() -> type["DeterministicAttentionMetadataBuilder"]:
+        return DeterministicAttentionMetadataBuilder
 
     @classmethod
     def supports_head_size(cls, head_size: int) -> bool:
@@ -73,6 +107,7 @@ class DeterministicAttentionImpl(AttentionImpl):
         self.frac_bits = cfg.frac_bits
         self.fxp_int_bits = cfg.fxp_int_bits
         self.num_kv_splits = cfg.num_kv_splits
+        self.fused_rope = cfg.fused_rope
         if alibi_slopes is not None:
             slopes = torch.tensor(alibi_slopes, dtype=torch.float32) * RCP_LN2
             assert slopes.shape == (num_heads,), \
@@ -100,15 +135,19 @@ class DeterministicAttentionImpl(AttentionImpl):
         if self.alibi_slopes is not None and self.alibi_slopes.device != query.device:
             self.alibi_slopes = self.alibi_slopes.to(query.device)
         n = attn_metadata.num_actual_tokens
-        unified_attention_fxp(
+        args = dict(
             q=query[:n], kv_cache=kv_cache, o=output[:n],
             query_start_loc=attn_metadata.query_start_loc, seq_lens=attn_metadata.seq_lens,
             block_table=attn_metadata.block_table, max_query_len=int(attn_metadata.max_query_len),
             alibi_slopes=self.alibi_slopes, fxp_dtype=self.fxp_int_bits, is_causal=True,
             softmax_scale=self.scale, frac_bits=self.frac_bits,
             logits_soft_cap=self.logits_soft_cap, window_size=self.window_size,
-            num_kv_splits=self.num_kv_splits, max_seq_len=int(attn_metadata.max_seq_len),
+            max_seq_len=int(attn_metadata.max_seq_len),
         )
+        if getattr(attn_metadata, "use_cascade", False):
+            shared_prefix_attention_fxp(common_prefix_len=int(attn_metadata.common_prefix_len), **args)
+        else:
+            unified_attention_fxp(num_kv_splits=self.num_kv_splits, **args)
         return output.view(num_tokens, self.num_heads * self.head_size)
 
     def do_kv_cache_update(self, layer: AttentionLayer, key: torch.Tensor, value: torch.Tensor,
@@ -120,3 +159,17 @@ class DeterministicAttentionImpl(AttentionImpl):
         key_cache, value_cache = kv_cache.unbind(1)
         reshape_and_cache_flash(key, value, key_cache, value_cache, slot_mapping,
                                 self.kv_cache_dtype, layer._k_scale, layer._v_scale)
+
+    def fused_rope_kvcache_supported(self) -> bool:
+        return self.fused_rope
+
+    def do_rope_and_kv_cache_update(self, layer: AttentionLayer, query: torch.Tensor, key: torch.Tensor,
+                                    value: torch.Tensor, positions: torch.Tensor,
+                                    cos_sin_cache: torch.Tensor, is_neox: bool, kv_cache: torch.Tensor,
+                                    layer_slot_mapping: torch.Tensor) -> None:
+        """Rotary position of query and key in place, key and value into the cache."""
+        n = query.shape[0]
+        q = query.view(n, self.num_heads, self.head_size)
+        k, v = (x.view(n, self.num_kv_heads, self.head_size) for x in (key, value))
+        rope_append_kv_fxp(q, k, v, kv_cache, layer_slot_mapping[:n], positions[:n], cos_sin_cache,
+                           is_neox, q_out=q, k_out=k)

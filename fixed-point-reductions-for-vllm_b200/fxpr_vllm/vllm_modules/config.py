@@ -69,6 +69,10 @@ _SWITCHES = {
     "enable_logprobs": "VLLM_FXP_DET_LOGPROBS",
     "enable_lm_head": "VLLM_FXP_DET_LM_HEAD",
 }
+# the same, default off
+_OPT_INS = {
+    "fused_rope": "VLLM_FXP_FUSED_ROPE",
+}
 _OFF_WORDS = frozenset({"0", "false", "no", "off"})
 
 
@@ -82,6 +86,7 @@ class FxpRuntimeConfig:
     enable_attn: bool = True
     enable_logprobs: bool = True
     enable_lm_head: bool = True
+    fused_rope: bool = False
 
 
 def _resolve_int(knob: _IntKnob, env: Mapping[str, str], got: Mapping[str, object]) -> int:
@@ -100,9 +105,9 @@ def _resolve_int(knob: _IntKnob, env: Mapping[str, str], got: Mapping[str, objec
     return value
 
 
-def _resolve_switch(name: str, env: Mapping[str, str]) -> bool:
+def _resolve_switch(name: str, env: Mapping[str, str], default: bool = True) -> bool:
     text = env.get(name, "")
-    return True if text == "" else text.strip().lower() not in _OFF_WORDS
+    return default if text == "" else text.strip().lower() not in _OFF_WORDS
 
 
 def load_runtime_config(env: Mapping[str, str] | None = None) -> FxpRuntimeConfig:
@@ -114,6 +119,8 @@ def load_runtime_config(env: Mapping[str, str] | None = None) -> FxpRuntimeConfi
         got[knob.field] = _resolve_int(knob, env, got)
     for field, name in _SWITCHES.items():
         got[field] = _resolve_switch(name, env)
+    for field, name in _OPT_INS.items():
+        got[field] = _resolve_switch(name, env, default=False)
     return FxpRuntimeConfig(**got)
 
 

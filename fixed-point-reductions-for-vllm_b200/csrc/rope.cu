@@ -14,26 +14,31 @@
 // norm and rotation as two operators round twice.
 //
 // Bound: HBM. Each row is read and written once. 8192 tokens, 32 + 8 heads x
-// 128, bf16: rotation and append 38.9 us for 204 MB (5.2 TB/s, 80% of a copy);
-// with the norm 41.5 us for 170 MB (4.1 TB/s, 63%): there the chain of square
-// sum, exchange, divide and square root of a row is not hidden by the 24 warps
-// that the registers leave room for.
+// 128, bf16: rotation and append 35.8 us for 204 MB (5.7 TB/s, 87% of a copy);
+// with the norm 34.4 us for 170 MB (4.9 TB/s, 76%): there 250 instructions a
+// lane and row keep the issue slots half busy as well.
 //
 // Layout of the vector kernel: a row belongs to a group of LPR lanes and each
 // lane holds two 8-value pieces, chosen so that both halves of a rotation pair
 // sit in one lane: no exchange but the integer sum of the squares. The groups
 // of a CTA are neighbouring tokens and the CTA walks a range of heads of one
-// of q, k and v, with the next two rows' loads in flight and its pieces of
-// cos, sin and the weights in registers throughout.
+// of q, k and v, with its pieces of cos, sin and the weights in registers
+// throughout; the next rows come by asynchronous copies into words of shared
+// memory that only the copying thread reads, which costs no registers and no
+// barrier.
 #include "fxp_common.cuh"
 
 namespace fxpr {
 namespace rope {
 
 constexpr int THREADS = 256;
-// resident CTAs per SM of the vector kernel (80 registers a thread), measured at 8192 tokens, 32 + 8 heads x 128, bf16, with
-// the norm / with the append: 2 CTAs 45.5 / 45.7 us, 3 CTAs 41.5 / 38.9 us, 4 CTAs (spills) 52.3 / 40.4 us
-constexpr int MINB = 3;
+// Resident CTAs per SM (64 registers a thread) and rows in flight per lane.
+// 8192 tokens, 32 + 8 heads x 128, bf16, with the norm / with the append: 3
+// CTAs 34.7 / 35.6 us, 4 CTAs 34.4 / 35.8 us, 5 CTAs (spills) 56.7 / 38.3 us;
+// 4 CTAs with 3 instead of 4 rows 35.7 / 37.0 us; two rows in registers
+// instead of the ring 41.5 / 38.9 us.
+constexpr int MINB = 4;
+template <typename T> constexpr int STAGES = sizeof(T) == 2 ? 4 : 2;
 
 struct Params {
   const void* x[3];  // q, k, v
@@ -220,25 +225,31 @@ __device__ __forceinline__ float2 turn2(float2 x, float2 c, float2 y, float2 s, 
 
 // The rows of one CTA: heads [0, n) from the pointers on, for this lane's
 // token and pieces. SQ: accumulator width of the norm, 0 = none.
+template <typename T> using Ring = uint4[STAGES<T>][2 * Piece<T>::N][THREADS];
+
 template <typename T, int SQ, int LPR, bool TURN>
-__device__ __forceinline__ void walk(const Params& p, int part, bool active, bool turn, int lo, int hi, const T* src,
+__device__ __forceinline__ void walk(const Params& p, Ring<T>& ring, int part, bool active, bool turn, int lo, int hi, const T* src,
                                      int64_t src_step, T* dst, int64_t dst_step, bool cached, int64_t cache_at,
                                      int64_t cache_step, int n, const float2 (&cs)[4], const float2 (&sn)[4]) {
   constexpr int BITS = SQ == 0 ? 32 : SQ;
   using UAcc = typename std::conditional<BITS == 64, unsigned long long, uint32_t>::type;
-  Piece<T> a0, b0, a1, b1;
-  a0.zero(); b0.zero(); a1.zero(); b1.zero();
+  // rows in flight: a ring of 16-byte words that only this thread reads
+  constexpr int NW = Piece<T>::N, S = STAGES<T>;
   const int gap = hi - lo;
   const T* next = src + lo;
-  auto fetch = [&](Piece<T>& a, Piece<T>& b, int h) {
+  auto fetch = [&](int h) {
     if (active && h < n) {
-      a.load(next);
-      b.load(next + gap);
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        cp_async16(&ring[h % S][i][threadIdx.x], reinterpret_cast<const uint4*>(next) + i, 16);
+        cp_async16(&ring[h % S][NW + i][threadIdx.x], reinterpret_cast<const uint4*>(next + gap) + i, 16);
+      }
     }
+    cp_async_commit();
     next += src_step;
   };
-  fetch(a0, b0, 0);
-  fetch(a1, b1, 1);
+#pragma unroll
+  for (int h = 0; h < S - 1; ++h) fetch(h);
   const float2 one = make_float2(p.one, p.one);
   float2 wa[4] = {}, wb[4] = {};
   float scale = 0.0f, thr = 0.0f;
@@ -302,23 +313,27 @@ __device__ __forceinline__ void walk(const Params& p, int part, bool active, boo
     }
     cat += cache_step;
   };
-  for (int h = 0; h < n; h += 2) {  // uniform over the CTA
-    {
-      const Piece<T> a = a0, b = b0;
-      fetch(a0, b0, h + 2);
-      row(a, b);
+  for (int h = 0; h < n; ++h) {  // uniform over the CTA
+    cp_async_wait<S - 2>();
+    Piece<T> a, b;
+    a.zero();
+    b.zero();
+    if (active) {
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        a.w[i] = ring[h % S][i][threadIdx.x];
+        b.w[i] = ring[h % S][NW + i][threadIdx.x];
+      }
     }
-    if (h + 1 < n) {
-      const Piece<T> a = a1, b = b1;
-      fetch(a1, b1, h + 3);
-      row(a, b);
-    }
+    fetch(h + S - 1);  // into the words read in the iteration before
+    row(a, b);
   }
 }
 
 // NORM: accumulator width of the norm, 0 = none
 template <typename T, int NORM, int LPR>
 __global__ void __launch_bounds__(THREADS, MINB) rope_vec_kernel(const __grid_constant__ Params p) {
+  __shared__ Ring<T> ring;
   const int64_t tok = (int64_t)(blockIdx.x / p.ranges) * (THREADS / LPR) + threadIdx.x / LPR;
   const int c = threadIdx.x % LPR;  // this lane's pair of pieces
   const bool active = tok < p.tokens && c < p.dim / 16;
@@ -347,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, MINB) rope_vec_kernel(const __grid_co
   const int64_t cache_step = part > 0 ? p.c_sh[part - 1] : 0;
   float2 cs[4], sn[4];
   if (part == 2) {
-    walk<T, 0, LPR, false>(p, 2, active, false, lo, hi, src, p.x_sh[2], nullptr, 0, slot >= 0, cache_at, cache_step, n, cs, sn);
+    walk<T, 0, LPR, false>(p, ring, 2, active, false, lo, hi, src, p.x_sh[2], nullptr, 0, slot >= 0, cache_at, cache_step, n, cs, sn);
     return;
   }
   const bool turn = active && c < rp;
@@ -362,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, MINB) rope_vec_kernel(const __grid_co
   }
   T* dst = reinterpret_cast<T*>(p.y[part]);
   if (dst != nullptr) dst += t * p.y_st[part] + h0 * p.y_sh[part];
-  walk<T, NORM, LPR, true>(p, part, active, turn, lo, hi, src, p.x_sh[part], dst, p.y_sh[part], slot >= 0, cache_at,
+  walk<T, NORM, LPR, true>(p, ring, part, active, turn, lo, hi, src, p.x_sh[part], dst, p.y_sh[part], slot >= 0, cache_at,
                            cache_step, n, cs, sn);
 }
 
@@ -430,8 +445,9 @@ __global__ void __launch_bounds__(THREADS) rope_any_kernel(const __grid_constant
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// Heads per CTA, halved while the CTAs do not fill the GPU. At the sizes above: 4 heads 45.5 / 42.2 us, 8 heads 41.5 / 38.9 us,
-// 16 heads 45.2 / 39.5 us; one token: one head per CTA, 3.0 us in a graph, 2 of which are the empty launch.
+// Heads per CTA, halved while the CTAs do not fill the GPU. At the sizes above
+// 16 heads 37.0 / 37.1 us; one token: one head per CTA, 3.1 us in a graph, 2
+// of which are the empty launch.
 constexpr int RANGE = 8;
 
 template <typename T, int NORM, int LPR>

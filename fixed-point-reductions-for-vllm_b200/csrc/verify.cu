@@ -30,9 +30,11 @@ namespace cg = cooperative_groups;
 namespace fxpr {
 namespace verify {
 
-// 256 threads, six CTAs per SM (40 registers), four loads of a lane in flight: 128 requests of 128256 fp32 entries, 81 of them
-// refusing (83 MB), 24.1 us (3.5 TB/s, 53% of a copy, of which about 8 us are the launch, the chain of reads that decides on
-// the drafted tokens, and the draw). 512 threads 24.8 to 31 us; fewer resident CTAs 35 us. One request: 4.7 us.
+// 256 threads, six CTAs per SM (40 registers), four 16-byte loads per tensor
+// of a lane in flight: 128 requests of 128256 fp32 entries, 81 of them refusing
+// (83 MB), 21.8 us (3.8 TB/s, 58% of a copy; about 8 us of it are the launch,
+// the chain of reads that decides on the drafted tokens, and the draw). Four or
+// five CTAs 23.4 to 24.6 us, 512 threads 25 us. One request: 3.9 us.
 constexpr int THREADS = 256;
 constexpr int MINB = 6;
 constexpr int UNROLL = 4;
@@ -178,14 +180,39 @@ __global__ void __launch_bounds__(THREADS, MINB) verify_kernel(const __grid_cons
   };
   auto sum_of = [&](bool all) -> u64 {
     u64 s = 0;
-#pragma unroll UNROLL
-    for (int64_t w = lo + lane * E; w < hi; w += 32 * E) {
-      uint32_t x[E];
-      entries(w, all, x);
+    auto add = [&](const uint32_t (&x)[E]) {
       // two entries are at most 2^31
 #pragma unroll
       for (int e = 0; e + 1 < E; e += 2) s += x[e] + x[e + 1];
       if (E == 1) s += x[0];
+    };
+    int64_t w = lo + lane * E;
+    if (w < shift && w < hi) {  // the row's first block, where it starts inside one
+      uint32_t x[E];
+      entries(w, all, x);
+      add(x);
+      w += 32 * E;
+    }
+    // whole turns: every block lies in the row, and UNROLL of them are in flight
+    for (; w + (UNROLL - 1) * 32 * E + E <= hi; w += UNROLL * 32 * E) {
+      Vec<T, E> a[UNROLL], b[UNROLL];
+#pragma unroll
+      for (int g = 0; g < UNROLL; ++g) {
+        a[g] = *reinterpret_cast<const Vec<T, E>*>(prow.base + w + g * 32 * E);
+        if constexpr (Q) b[g] = *reinterpret_cast<const Vec<T, E>*>(qrow.base + w + g * 32 * E);
+      }
+#pragma unroll
+      for (int g = 0; g < UNROLL; ++g) {
+        uint32_t x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = left_of<T, Q>(a[g].v[e], b[g].v[e], w + g * 32 * E + e, mark, scale, all);
+        add(x);
+      }
+    }
+    for (; w < hi; w += 32 * E) {
+      uint32_t x[E];
+      entries(w, all, x);
+      add(x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -275,7 +302,7 @@ template <typename T, bool Q, int E>
 static int launch(Params p, int64_t requests, cudaStream_t st) {
   // CTAs per request: what is resident at once over the batch, or somewhat
   // more, since requests that refuse nothing leave early (two per SM 44 us,
-  // eight 24 us at the batch above); each with at least one turn of its warps
+  // eight 24 us at the batch above, before the whole-turn loop); each with at least one turn of its warps
   int ranks = MAX_CLUSTER;
   while (ranks > 1 && (requests * ranks > 8 * num_sms() || (int64_t)(ranks / 2) * THREADS * E >= p.vocab)) ranks /= 2;
   p.span = cdiv(cdiv(p.vocab + E, (int64_t)ranks * WARPS), 32 * E) * 32 * E;  // the shift is below E

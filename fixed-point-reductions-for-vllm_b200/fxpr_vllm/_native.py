@@ -7,7 +7,6 @@ device, the call raises.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -173,31 +172,35 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
-def same_device(*tensors: torch.Tensor | None) -> torch.device:
-    """The one CUDA device of all given tensors; raises if there are several."""
-    dev = None
+def same_device(*tensors: torch.Tensor | None) -> int:
+    """The index of the one CUDA device of all given tensors; raises if they
+    are not on CUDA, or on several devices."""
+    index = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError("fxpr_vllm kernels require CUDA tensors (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    return dev
+        i = t.get_device()
+        if i != index:
+            if i < 0:
+                raise RuntimeError("fxpr_vllm kernels require CUDA tensors (no CPU fallback)")
+            if index is not None:
+                raise ValueError(f"tensors on different devices: cuda:{index} and cuda:{i}")
+            index = i
+    return index
 
 
-def on_device(device: torch.device):
-    """Context in which kernels launch on ``device``, whichever device is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def launch(fn, index: int, *args) -> int:
+    """``fn(*args, stream)`` on CUDA device ``index`` and its current stream,
+    whichever device is current."""
+    stream = torch._C._cuda_getCurrentRawStream(index)  # without a Stream object around it
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, stream)
+    with torch.cuda.device(index):
+        return fn(*args, stream)
 
 
 def stream_ptr(device: torch.device) -> int:
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    return torch._C._cuda_getCurrentRawStream(index)  # without a Stream object around it
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def dcode(t: torch.Tensor) -> int:

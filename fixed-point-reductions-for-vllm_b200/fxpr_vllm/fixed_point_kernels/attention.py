@@ -221,10 +221,10 @@ def shared_prefix_attention_fxp(
     p.logits_soft_cap = logits_soft_cap * RCP_LN2 if logits_soft_cap > 0.0 else 0.0
     p.frac_bits, p.int_bits, p.num_kv_splits = frac_bits, int_bits_of(fxp_dtype), 8
     lib = N.load()
-    with N.on_device(dev):
-        need = lib.fxpr_shared_prefix_attention_workspace_bytes(ctypes.byref(p), common_prefix_len, tokens)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        if need:
-            p.workspace, p.workspace_bytes = ws.data_ptr(), need
-        rc = lib.fxpr_shared_prefix_attention_fxp(ctypes.byref(p), common_prefix_len, tokens, N.stream_ptr(dev))
-    N.check(rc, what)
+    need = lib.fxpr_shared_prefix_attention_workspace_bytes(ctypes.byref(p), common_prefix_len, tokens)
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+    if need:
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    rc = N.launch(lib.fxpr_shared_prefix_attention_fxp, dev, ctypes.byref(p), common_prefix_len, tokens)
+    if rc:
+        N.check(rc, what)

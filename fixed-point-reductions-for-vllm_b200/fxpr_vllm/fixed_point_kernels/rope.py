@@ -71,7 +71,7 @@ def _params(what: str, q, k, positions, cos_sin_cache, is_neox, q_weight, k_weig
 
 def _out(what: str, name: str, out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(like.shape)
     if out.shape != like.shape or out.dtype != like.dtype or (out.stride(-1) != 1 and out.shape[-1] != 1):
         raise ValueError(f"{what}: {name} must have the input's shape and type, with head_dim contiguous")
     return out
@@ -99,9 +99,9 @@ def qk_norm_rope_fxp(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k
     p.qo_stride_tok, p.qo_stride_head, _ = yq.stride()
     p.ko_stride_tok, p.ko_stride_head, _ = yk.stride()
     dev = N.same_device(q, k, q_weight, k_weight, positions, cos_sin_cache, yq, yk)
-    with N.on_device(dev):
-        rc = N.load().fxpr_qk_norm_rope_fxp(ctypes.byref(p), N.stream_ptr(dev))
-    N.check(rc, what)
+    rc = N.launch(N.load().fxpr_qk_norm_rope_fxp, dev, ctypes.byref(p))
+    if rc:
+        N.check(rc, what)
     return yq, yk
 
 
@@ -151,7 +151,7 @@ def rope_append_kv_fxp(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cac
     p.num_blocks, p.page_size = cs[0], cs[2]
     p.slot_mapping, p.num_slots = slots.data_ptr(), slots.shape[0]
     dev = N.same_device(q, k, v, kv_cache, slot_mapping, positions, cos_sin_cache, q_weight, k_weight, yq, k_out)
-    with N.on_device(dev):
-        rc = N.load().fxpr_rope_append_kv_fxp(ctypes.byref(p), N.stream_ptr(dev))
-    N.check(rc, what)
+    rc = N.launch(N.load().fxpr_rope_append_kv_fxp, dev, ctypes.byref(p))
+    if rc:
+        N.check(rc, what)
     return yq

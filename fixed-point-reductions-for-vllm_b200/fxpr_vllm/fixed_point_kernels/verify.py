@@ -73,13 +73,13 @@ def verify_draft_fxp(target_probs: torch.Tensor, draft_probs: torch.Tensor | Non
     ids, bonus = draft_token_ids.contiguous(), bonus_token_ids.contiguous()
     start = draft_start_loc.to(torch.int32).contiguous()
     u, r = accept_uniform.contiguous(), resample_uniform.contiguous()
-    out = torch.empty((reqs, most + 1), dtype=torch.int32, device=dev)
-    taken = torch.empty((reqs,), dtype=torch.int32, device=dev)
-    with N.on_device(dev):
-        rc = N.load().fxpr_verify_draft_fxp(
-            p.data_ptr(), None if q is None else q.data_ptr(), N.DTYPE_CODE[p.dtype], p.stride(0),
-            0 if q is None else q.stride(0), n, vocab, ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0,
-            start.data_ptr(), bonus.data_ptr(), 1 if bonus.dtype == torch.int64 else 0, u.data_ptr(), r.data_ptr(),
-            reqs, most, f, out.data_ptr(), most + 1, taken.data_ptr(), N.stream_ptr(dev))
-    N.check(rc, "verify_draft_fxp")
+    out = p.new_empty((reqs, most + 1), dtype=torch.int32)
+    taken = p.new_empty((reqs,), dtype=torch.int32)
+    rc = N.launch(
+        N.load().fxpr_verify_draft_fxp, dev, p.data_ptr(), None if q is None else q.data_ptr(), N.DTYPE_CODE[p.dtype],
+        p.stride(0), 0 if q is None else q.stride(0), n, vocab, ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0,
+        start.data_ptr(), bonus.data_ptr(), 1 if bonus.dtype == torch.int64 else 0, u.data_ptr(), r.data_ptr(),
+        reqs, most, f, out.data_ptr(), most + 1, taken.data_ptr())
+    if rc:
+        N.check(rc, "verify_draft_fxp")
     return out, taken

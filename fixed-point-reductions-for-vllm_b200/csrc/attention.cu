@@ -935,6 +935,7 @@ extern "C" int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* a, 
   p.ws_s = reinterpret_cast<float*>(ws + pp.off_s);
   p.nchunk_max = pp.nchunk;
   p.key0 = pp.key0;
+  p.tokens = num_tokens;
   float* scores = reinterpret_cast<float*>(ws + pp.off_p);
   if (cudaMemsetAsync(ws, 0, pp.off_s, st) != cudaSuccess) return check_launch("fxpr_shared_prefix_attention_fxp (clear)");
   rc = attn::launch_suffix(p, false, a->head_dim, pl.rp, a->int_bits, a->kv_dtype, a->num_requests, pl.ys, st);

@@ -231,7 +231,11 @@ __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
   if constexpr (PRE) launch_dependents();
   int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
   if (kr_hi < 0) return;  // uniform over the CTA
-  if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
+  if constexpr (PRE) {
+    kr_hi = max(kr_hi, p.key0);
+    if (threadIdx.x < RP && row_tok[threadIdx.x] >= p.tokens) row_tok[threadIdx.x] = -1;  // no such row of q
+    __syncthreads();
+  }
   const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
   if (chunk > 0 && kb >= kr_hi) return;
   const int ke = min(kb + CHUNK, kr_hi);
@@ -396,7 +400,7 @@ __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
 // once and q never is; the 8 partial dots of (2 keys x 4 rows) are
 // reduce-scattered over the 8 lanes, one score per lane.
 // ---------------------------------------------------------------------------
-template <int D, int BITS, typename KVT, bool PL, bool PRE = false>
+template <int D, int BITS, typename KVT, bool PL>
 __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
   constexpr int RP = 4;
   using TL = Tile<D, KVT, KTC>;
@@ -426,11 +430,9 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
   const int kvh = blockIdx.y / p.head_slices, hslice = blockIdx.y % p.head_slices;
   const int req = blockIdx.z / p.qtiles, qtile = blockIdx.z % p.qtiles;
   if (t == 0) q_or = 0u;
-  int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
-  if (kr_hi < 0) return;  // uniform over the CTA
-  if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
-  const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
-  if (chunk > 0 && kb >= kr_hi) return;
+  const int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
+  const int kb = chunk * CHUNK;
+  if (kr_hi < 0 || (chunk > 0 && kb >= kr_hi)) return;  // uniform over the CTA
   const int ke = min(kb + CHUNK, kr_hi);
   const int ntiles = (ke - kb + KTC - 1) / KTC;
   const int64_t item = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
@@ -446,7 +448,7 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
     cp_async_commit();
   }
   int next_blk = (NBS - 1 < ntiles) ? cp.block_of(NBS - 1) : -1;
-  if constexpr (!PRE) clear_item<RP, D>(p, item, chunk, kr_hi);
+  clear_item<RP, D>(p, item, chunk, kr_hi);
   const float kthr = stage_q<RP, D>(p, row_tok, row_head, q_s, q_raw, &q_or, scale);
 
   // this thread's q (pre-scaled), as fp32 pairs
@@ -633,11 +635,7 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
     float m = -INFINITY;
 #pragma unroll
     for (int w2 = 0; w2 < THREADS / 32; ++w2) m = fmaxf(m, wmax[w2][t]);
-    if constexpr (PRE) {
-      if (row_tok[t] >= 0) atomicMax(&p.row_max[(int64_t)row_tok[t] * p.num_heads + row_head[t]], ordered(m));
-    } else {
-      p.ws_m[unit * RP + t] = m;
-    }
+    p.ws_m[unit * RP + t] = m;
   }
 }
 
@@ -677,7 +675,11 @@ __global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_ker
     if constexpr (PRE) wait_dependencies();  // the launch ends after the one it overlaps
     return;
   }
-  if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
+  if constexpr (PRE) {
+    kr_hi = max(kr_hi, p.key0);
+    if (threadIdx.x < RP && row_tok[threadIdx.x] >= p.tokens) row_tok[threadIdx.x] = -1;  // no such row of q
+    __syncthreads();
+  }
   const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
   if (chunk > 0 && kb >= kr_hi) {
     if constexpr (PRE) wait_dependencies();

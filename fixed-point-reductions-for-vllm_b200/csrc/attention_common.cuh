@@ -56,6 +56,7 @@ struct Params {
   // shared-prefix form: keys before key0 belong to the prefix kernels
   // (attention_prefix.cu); rows are token * num_heads + head
   int key0;
+  int64_t tokens;               // rows of q and o
   uint32_t* row_max;            // [rows] row maxima over all keys, as ordered integers
   unsigned long long* row_den;  // [rows] integer normaliser partial sums
   unsigned long long* row_acc;  // [rows][D] integer PV partial sums

@@ -302,3 +302,34 @@ def test_captured_and_on_another_stream():
     side.synchronize()
     assert bits_equal(yq, y2) and bits_equal(kv.flatten(0, 1)[2:3], want.flatten(0, 1)[2:3])
     assert torch.equal(kv[1:], want[1:])
+
+
+@pytest.mark.gpu
+def test_append_offsets_beyond_32_bits():
+    """Slots whose offsets in the cache pass 2^31 elements, in the vector kernel and the general one."""
+    for D in (64, 40):
+        q, k, v, _, _, pos, tab = _inputs(5, 2, 1, D, 8, torch.bfloat16, seed=9, device="cuda")
+        blocks = 2**31 // (2 * 16 * D) + 4
+        kv = torch.empty(blocks, 2, 16, 1, D, dtype=torch.bfloat16, device="cuda")
+        kv[-3:] = 0
+        small = torch.zeros(3, 2, 16, 1, D, dtype=torch.bfloat16, device="cuda")
+        slots = torch.tensor([3, 20, 47, 0, 31], device="cuda")
+        R.rope_append_kv_fxp(q, k, v, kv, slots + 16 * (blocks - 3), pos, tab)
+        R.rope_append_kv_fxp(q, k, v, small, slots, pos, tab)
+        assert bits_equal(kv[-3:].contiguous(), small) and (small != 0).any()
+
+
+@pytest.mark.gpu
+def test_the_same_call_on_two_streams_at_once():
+    """Two calls in flight at the same time share nothing but their inputs."""
+    q, k, v, qw, kw, pos, tab = _inputs(2000, 16, 4, 128, 128, torch.bfloat16, seed=10, device="cuda")
+    want = R.qk_norm_rope_fxp(q, k, qw, kw, pos, tab)
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, g in zip(streams, got):
+            with torch.cuda.stream(s):
+                g.append(R.qk_norm_rope_fxp(q, k, qw, kw, pos, tab))
+    torch.cuda.synchronize()
+    for a, b in got[0] + got[1]:
+        assert bits_equal(a, want[0]) and bits_equal(b, want[1])

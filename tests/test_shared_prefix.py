@@ -115,6 +115,7 @@ def test_abi_refuses_and_sizes_its_workspace():
     ([5, 1, 3, 9, 2], [5, 8, 3, 30, 2], 333, 8, 4, 8),       # verification, group of 2, small pages
     ([70, 1, 130], [70, 1, 200], 704, 7, 1, 48),             # chunked prefill, group of 7, pages across tiles
     ([1], [3], 500, 16, 2, 16),                              # one request
+    ([1, 2, 1], [3, 900, 20], 397, 6, 2, 5),                 # pages of an odd number of keys
     ([2, 0, 3, 0], [2, 0, 9, 5], 290, 2, 2, 1),              # requests without queries, pages of one key
 ])
 def test_bits_of_the_unified_attention(qlens, suffix, prefix, H, KVH, page, D, bits):
@@ -126,7 +127,8 @@ def test_bits_of_the_unified_attention(qlens, suffix, prefix, H, KVH, page, D, b
 @pytest.mark.gpu
 @pytest.mark.parametrize("kw", [dict(logits_soft_cap=20.0), dict(window_size=100), dict(window_size=3), dict(is_causal=False),
                                 dict(window_size=400, logits_soft_cap=5.0), dict(softmax_scale=0.3), dict(alibi=True),
-                                dict(alibi=True, window_size=300), dict(frac_bits=8), dict(frac_bits=20)])
+                                dict(alibi=True, window_size=300), dict(frac_bits=8), dict(frac_bits=20), dict(frac_bits=0),
+                                dict(frac_bits=30)])
 @pytest.mark.parametrize("qlens, suffix", [([1] * 12, [1 + 40 * (r % 3) for r in range(12)]), ([6, 1, 3], [60, 1, 3])])
 def test_masks_and_scores(kw, qlens, suffix):
     kw = dict(kw)
@@ -230,6 +232,9 @@ def test_strides_types_and_other_forms():
     tab[:, ::3] = bt
     A.shared_prefix_attention_fxp(wide[:, 1], store, out[:, :, 1], qsl.long(), sl.long(), tab[:, ::3], 384, mq)
     assert bits_equal(out[:, :, 1].contiguous(), want) and (out[:, :, 0] == 0).all()
+    odd = torch.zeros(6, 8, 67, dtype=BF, device="cuda")
+    odd[..., 1:65] = q
+    _same(((odd[..., 1:65], kv, qsl, sl, bt), mq, ms), 384)
     for o_dtype in (BF, HF):
         a, b = _pair(((q, kv, qsl, sl, bt), mq, ms), 384, o_dtype=o_dtype)
         assert bits_equal(a, b)
@@ -273,6 +278,29 @@ def test_batch_invariance_and_repeat():
         out.zero_()
         run(i, n)
         assert bits_equal(out[:n], full[i:i + n])
+
+
+@pytest.mark.gpu
+def test_query_ranges_behind_the_queries():
+    """A last request whose range ends behind the rows of q: its missing rows are skipped, the others keep their bits."""
+    (q, kv, qsl, sl, bt), mq, ms = _batch([1] * 18 + [6], [5] * 18 + [9], 256, 8, 4, 128, seed=19)
+    want = _same(((q, kv, qsl, sl, bt), mq, ms), 256)
+    guard = torch.full((40, 8, 128), 7.0, device="cuda")
+    A.shared_prefix_attention_fxp(q[:20], kv, guard[:20], qsl, sl, bt, 256, mq, max_seq_len=ms)
+    assert bits_equal(guard[:20], want[:20]) and (guard[20:] == 7.0).all()
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Pages whose offsets in the cache pass 2^31 elements (a 4.7 GB cache of which a few pages are written)."""
+    (q, kv, qsl, sl, bt), mq, ms = _batch([1] * 6, [9] * 6, 256, 16, 8, 128, seed=20)
+    want = _same(((q, kv, qsl, sl, bt), mq, ms), 256)
+    far = 2**31 // (2 * 16 * 8 * 128) + 1
+    big = torch.empty(far + kv.shape[0] + 1, 2, 16, 8, 128, dtype=BF, device="cuda")
+    big[far:far + kv.shape[0]] = kv
+    out = torch.zeros(q.shape, device="cuda")
+    A.shared_prefix_attention_fxp(q, big, out, qsl, sl, bt + far, 256, mq, max_seq_len=ms)
+    assert bits_equal(out, want)
 
 
 @pytest.mark.gpu

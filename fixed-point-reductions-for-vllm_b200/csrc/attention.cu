@@ -780,6 +780,19 @@ constexpr int kPrefixMinKeys = 256;
 constexpr int64_t kPrefixMinDecodePairs = 2ll << 20;
 constexpr int64_t kPrefixScores = 128ll << 20;  // about the L2
 
+// Rows per tile: the least total of tiles times a tile's cost, 0.6 : 1 : 1.95
+// for 16 : 32 : 64 rows. Measured behind 4096 keys, 8 KV heads, head_dim 128
+// (64), us with 16 / 32 / 64 rows: 24 rows a KV head 52 / 46 / - (37 / 30 / -),
+// 40 rows 70 / 74 / 72 (48 / 45 / 44), 64 rows 86 / 77 / 77 (58 / 47 / 46), 72
+// rows 102 / 102 / 122 (68 / 61 / 69), 130 rows 174 / 158 / 177 (114 / 93 / 100).
+int prefix_row_tile(int64_t rows) {
+  int best = 64;
+  int64_t least = cdiv(rows, 64) * 195;
+  if (cdiv(rows, 32) * 100 < least) best = 32, least = cdiv(rows, 32) * 100;
+  if (cdiv(rows, 16) * 60 < least) best = 16;
+  return best;
+}
+
 struct PrefixPlan {
   bool use;
   int key0, row_tile, tiles, pass_tiles, nchunk;
@@ -802,7 +815,7 @@ PrefixPlan prefix_plan_of(const fxpr_attention_params* a, int prefix_len, int64_
   auto fits = [](int64_t s) { return s >= 0 && s <= 0x7fffffffLL; };
   if (!fits(a->k_stride_blk) || !fits(a->k_stride_slot) || !fits(a->v_stride_blk) || !fits(a->v_stride_slot)) return pp;
   pp.key0 = key0;
-  pp.row_tile = rows_kv <= 16 ? 16 : rows_kv <= 32 ? 32 : 64;
+  pp.row_tile = prefix_row_tile(rows_kv);
   const int64_t tiles = cdiv(rows_kv, pp.row_tile);
   pp.nchunk = (int)cdiv(pl.max_keys - key0, attn::CHUNK);
   if (pp.nchunk < 1) pp.nchunk = 1;

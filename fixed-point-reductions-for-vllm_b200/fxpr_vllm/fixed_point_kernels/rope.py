@@ -71,7 +71,7 @@ def _params(what: str, q, k, positions, cos_sin_cache, is_neox, q_weight, k_weig
 
 def _out(what: str, name: str, out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return like.new_empty(like.shape)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if out.shape != like.shape or out.dtype != like.dtype or (out.stride(-1) != 1 and out.shape[-1] != 1):
         raise ValueError(f"{what}: {name} must have the input's shape and type, with head_dim contiguous")
     return out

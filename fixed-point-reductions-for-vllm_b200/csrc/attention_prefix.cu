@@ -417,9 +417,6 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
   const float vthr = __double2float_rd(fmin(65504.5, 4194304.0 / (scale_d * (1.0 + 1.0 / 1024))));
   const float2 C2 = make_float2(kMagic, kMagic), ONE2 = make_float2(p.one, p.one);
   const bool small_frac = p.frac <= 22;  // p * 2^f <= 2^22: the magic constant rounds it
-  // bf16 -> fp16 is exact from 2^-17 up to 65504, and below |p * v * 2^f| < 1/2 either way when f <= 16; beyond 65504
-  // (infinite in fp16) the tile is not fast and its V is converted again
-  const bool v_exact16 = std::is_same<T, __half>::value || p.frac <= 16;
   const int prow = t / TPR;             // p phase: this row, keys 4 * (t % TPR) + 4 * TPR * u
   const int dl = t % LD, grp = t / LD;  // this thread's dims 4 * dl.., rows grp * TM..
   const int vc = dl / 2, vj = (dl & 1) * 2, vx = (vc >> 1) & 3;
@@ -595,7 +592,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
               const float ps = pb[i * P_LD + k];
               if (__float_as_uint(ps) == 0x80000000u) continue;
               const float vv = reinterpret_cast<const float*>(vs + (size_t)(k / 2) * D * 8 + (e < 2 ? v0 : v1))[2 * (e & 1) + (k & 1)];
-              s += (UAcc)f2x_scaled<BITS>(__fmul_rn(ps, __half2float(__float2half_rn(vv))));
+              s += (UAcc)f2x_scaled<BITS>(__fmul_rn(ps, vv));
             }
             if (s) atomicAdd(p.row_acc + ((int64_t)rows.tok[r] * p.num_heads + rows.head[r]) * D + 4 * dl + e, (unsigned long long)s);
           }

@@ -161,8 +161,8 @@ def _(acc, bias, residual, weight, eps, frac_bits, fxp_int_bits):
 
 # The operators of a decode step below are registered through torch.library's
 # define/impl interface: the same namespace, schema checks and tracing as the
-# ones above, at about a quarter of their host time per call (4 instead of 14
-# to 27 us on this build's host), which is what a step of one token waits for.
+# ones above, at about a quarter of the host time per call (4 instead of 14 to
+# 27 us), which is what an uncaptured step of one token waits for.
 _lib = torch.library.Library("fxpr", "FRAGMENT")
 
 

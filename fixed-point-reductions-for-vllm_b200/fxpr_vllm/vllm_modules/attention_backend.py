@@ -33,17 +33,25 @@ logger = logging.getLogger("fxpr_vllm")
 
 
 class DeterministicAttentionMetadataBuilder(TritonAttentionMetadataBuilder):
-    """The Triton backend's metadata, with cascade attention from a common
-    prefix of ``MIN_PREFIX`` keys on (below, the shared-prefix operator runs
-    the unified kernels anyway)."""
+    """The Triton backend's metadata, with cascade attention for the steps that
+    the shared-prefix kernels take: a common prefix of ``MIN_PREFIX`` keys, and
+    ``MIN_DECODE_PAIRS`` (row, key) pairs where the decode kernels would run
+    otherwise (one query a request, four query heads a KV head). For the others
+    the operator runs the unified kernels, and the engine would only lose its
+    full CUDA graph."""
 
     MIN_PREFIX = 256
+    MIN_DECODE_PAIRS = 2 << 20
 
     def use_cascade_attention(self, common_prefix_len: int, query_lens, num_query_heads: int,
                               num_kv_heads: int, use_alibi: bool, use_sliding_window: bool,
                               use_local_attention: bool, num_sms: int, dcp_world_size: int) -> bool:
-        return (common_prefix_len >= self.MIN_PREFIX and len(query_lens) > 1
-                and not use_local_attention and dcp_world_size <= 1)
+        if (common_prefix_len < self.MIN_PREFIX or len(query_lens) < 2 or use_local_attention
+                or dcp_world_size > 1):
+            return False
+        rows = int(sum(query_lens)) * num_query_heads
+        decode = max(query_lens) == 1 and num_query_heads == 4 * num_kv_heads
+        return not decode or rows * common_prefix_len >= self.MIN_DECODE_PAIRS
 
     def build(self, common_prefix_len: int, common_attn_metadata, fast_build: bool = False):
         # the Triton builder's own cascade fields are not used (it leaves some

@@ -27,14 +27,16 @@ def test_fused_rope_is_opt_in():
     assert load_runtime_config({"VLLM_FXP_FUSED_ROPE": "off"}).fused_rope is False
 
 
-def test_backend_takes_cascade_for_long_prefixes_only():
+def test_backend_takes_cascade_where_the_prefix_kernels_run():
     from fxpr_vllm.vllm_modules.attention_backend import DeterministicAttentionBackend
 
     cls = DeterministicAttentionBackend.get_builder_cls()
-    ask = lambda n, lens, local=False, dcp=1: cls.use_cascade_attention(  # noqa: E731
-        cls.__new__(cls), n, lens, 32, 8, False, False, local, 148, dcp)
-    assert ask(256, [1, 1]) and ask(4096, [5, 1, 1])
-    assert not ask(255, [1, 1]) and not ask(4096, [1]) and not ask(4096, [1, 1], local=True) and not ask(4096, [1, 1], dcp=2)
+    ask = lambda n, lens, heads=32, local=False, dcp=1: cls.use_cascade_attention(  # noqa: E731
+        cls.__new__(cls), n, lens, heads, 8, False, False, local, 148, dcp)
+    assert ask(4096, [5, 1, 1]) and ask(256, [1, 1], heads=64) and ask(4096, [1] * 16)
+    assert not ask(4096, [1] * 15) and not ask(1024, [1, 1])  # decode batches with few (row, key) pairs
+    assert not ask(255, [5, 1]) and not ask(4096, [5]) and not ask(4096, [5, 1], local=True)
+    assert not ask(4096, [5, 1], dcp=2)
 
 
 def _impl(heads, kv_heads, dim):

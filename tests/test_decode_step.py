@@ -185,3 +185,40 @@ def test_engine_with_cascade_attention(tmp_path):
     assert got[True]["calls"] == [] and got[False]["calls"]
     assert all(n >= 256 for n in got[False]["calls"])
     assert got[True]["streams"] == got[False]["streams"]
+
+
+@pytest.mark.gpu
+def test_schemas_and_tracing():
+    """The operators' schemas name what they change, their shapes can be traced, and a compiled function gives their bits."""
+    g = torch.Generator().manual_seed(5)
+    ops = torch.ops.fxpr
+    x = torch.randn(6, 14, 64, generator=g).bfloat16().cuda()
+    q, k, v = x[:, :10], x[:, 10:12], x[:, 12:]
+    w, pos, tab = torch.ones(64, dtype=torch.bfloat16, device="cuda"), torch.arange(6, device="cuda"), torch.randn(9, 64, generator=g).cuda()
+    kv = torch.randn(24, 2, 16, 2, 64, generator=g).bfloat16().cuda()
+    bt = torch.cat([torch.arange(17).expand(3, -1), 17 + torch.arange(3)[:, None]], 1).int().cuda()
+    qsl = torch.tensor([0, 2, 4, 6], dtype=torch.int32, device="cuda")
+    sl = torch.full((3,), 280, dtype=torch.int32, device="cuda")
+    p = torch.softmax(torch.randn(6, 33, generator=g), -1).cuda()
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    u = torch.rand(6, generator=g).cuda()
+    calls = {
+        ops.qk_norm_rope_fxp.default: (q, k, w, w, pos, tab, True, 1e-6, 16, 32),
+        ops.rope_append_kv_fxp.default: (q, k, v, kv, pos + 275, pos, tab, False, None, None, 1e-6, 16, 32),
+        ops.shared_prefix_attention_fxp.default: (q, kv, torch.zeros_like(q), qsl, sl, bt, 272, 2, None, 32, True, None, 16, 0.0, 0, 280),
+        ops.verify_draft_fxp.default: (p, None, i32(1, 2, 3, 4, 5, 6), i32(0, 3, 6), i32(7, 8), u, u[:2], 3, 30),
+    }
+    for op, args in calls.items():
+        torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+    def step(q, k, v, kv, o):
+        q, k = ops.qk_norm_rope_fxp(q, k, w, w, pos, tab, True, 1e-6, 16, 32)
+        q = ops.rope_append_kv_fxp(q, k, v, kv, pos + 275, pos, tab, True, None, None, 1e-6, 16, 32)
+        ops.shared_prefix_attention_fxp(q, kv, o, qsl, sl, bt, 272, 2, None, 32, True, None, 16, 0.0, 0, 280)
+        return q, o.clone(), kv.clone()
+
+    fresh = lambda: (q, k, v, kv.clone(), torch.zeros(q.shape, device="cuda"))  # noqa: E731
+    want = step(*fresh())
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(*fresh())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

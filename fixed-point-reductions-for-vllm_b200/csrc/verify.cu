@@ -32,9 +32,9 @@ namespace verify {
 
 // 256 threads, six CTAs per SM (40 registers), four 16-byte loads per tensor
 // of a lane in flight: 128 requests of 128256 fp32 entries, 81 of them refusing
-// (83 MB), 21.8 us (3.8 TB/s, 58% of a copy; about 8 us of it are the launch,
+// (83 MB), 21.4 us (3.9 TB/s, 59% of a copy; about 8 us of it are the launch,
 // the chain of reads that decides on the drafted tokens, and the draw). Four or
-// five CTAs 23.4 to 24.6 us, 512 threads 25 us. One request: 3.9 us.
+// five CTAs 2 to 3 us more, 512 threads 3 us. One request: 3.8 us.
 constexpr int THREADS = 256;
 constexpr int MINB = 6;
 constexpr int UNROLL = 4;
@@ -123,8 +123,10 @@ __global__ void __launch_bounds__(THREADS, MINB) verify_kernel(const __grid_cons
   __shared__ u64 cta_sum;  // read by the other CTAs of the cluster
   __shared__ int s_taken;
   __shared__ bool s_refused;
+  __shared__ int64_t s_token;
 
   // ---- the drafted tokens: one lane per position ----
+  const u64 R = draw_of(p.r[req]);  // asked for ahead of its use
   const int64_t first = p.start[req];
   const int64_t length = min((int64_t)p.start[req + 1] - first, (int64_t)p.most);
   if (warp == 0) {
@@ -146,6 +148,7 @@ __global__ void __launch_bounds__(THREADS, MINB) verify_kernel(const __grid_cons
       s_taken = n;
       s_refused = refused != 0;
     }
+    if (refused && lane == n) s_token = id;
     if (rank == 0) {
       int32_t* o = p.out + req * p.out_stride;
       for (int i = lane; i <= p.most; i += 32) {
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(THREADS, MINB) verify_kernel(const __grid_cons
   if (!s_refused) return;  // uniform over the cluster
   const int64_t row = first + s_taken;
   const bool exists = row >= 0 && row < p.total;
-  const int64_t token = exists ? load_id(p.ids, p.ids64, row) : -1;
+  const int64_t token = s_token;
   const T* pr = reinterpret_cast<const T*>(p.p) + (exists ? row : 0) * p.p_stride;
   const int shift = E == 1 ? 0 : (int)((uintptr_t)pr % (E * sizeof(T)) / sizeof(T));
   const Row<T, E> prow = {pr - shift};
@@ -234,16 +237,21 @@ __global__ void __launch_bounds__(THREADS, MINB) verify_kernel(const __grid_cons
       if (c < rank) before += s;
       total += s;
     }
-    cluster.sync();  // nobody leaves or overwrites its sum while others read it
+    cluster.barrier_arrive();
   };
+  // nobody leaves or overwrites its sum while others may read it
+  auto part = [&]() { cluster.barrier_wait(); };
   bool all = false;
   meet(sum_of(false));
   if (total == 0) {  // uniform over the cluster: nothing remains, draw from the target itself
     all = true;
+    part();
     meet(sum_of(true));
   }
-  if (total == 0) return;  // no probability at all: -1 stays
-  const u64 R = draw_of(p.r[req]);
+  if (total == 0) {  // no probability at all: -1 stays
+    part();
+    return;
+  }
   const u64 goal = (total >> 24) * R + (((total & 0xFFFFFFull) * R) >> 24);
 
   // ---- the CTA that holds the goal looks through the share it lies in, one
@@ -254,7 +262,10 @@ __global__ void __launch_bounds__(THREADS, MINB) verify_kernel(const __grid_cons
     if (goal >= run && goal < run + warp_sum[w]) share = w;
     else run += warp_sum[w];
   }
-  if (share < 0) return;
+  if (share < 0) {
+    part();
+    return;
+  }
   const int64_t from = ((int64_t)rank * WARPS + share) * p.span;
   const int turns = (int)(p.span / (32 * E));
   for (int t0 = 0; t0 < turns; t0 += WARPS) {
@@ -290,9 +301,10 @@ __global__ void __launch_bounds__(THREADS, MINB) verify_kernel(const __grid_cons
         }
       p.out[req * p.out_stride + s_taken] = (int32_t)(w + e - shift);
     }
-    if (goal < run) return;  // uniform over the CTA
+    if (goal < run) break;  // uniform over the CTA
     __syncthreads();  // turn_sum is read
   }
+  part();
 }
 
 // ---------------------------------------------------------------------------

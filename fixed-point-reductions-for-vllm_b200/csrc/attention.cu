@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
     const int qoff = qtile * p.qt + qi;
     const int hg = hslice * p.gs + gh;
     int tok = -1, kend = 0, pos = 0, head = 0;
-    if (qi < p.qt && qoff < qlen && hg < p.group) {
+    if (qi < p.qt && qoff < qlen && hg < p.group && q_start + qoff < p.tokens) {
       tok = q_start + qoff;
       head = kvh * p.group + hg;
       pos = ctx + qoff;
@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
     const int j = kb + ti * KT + my_jl;
     if (j >= ke) return -1;
     const int bi = p.page_shift >= 0 ? (j >> p.page_shift) : j / p.page;
-    return p.bt[bt_row + bi];
+    const int b = p.bt[bt_row + bi];
+    return b < p.blocks ? b : -1;
   };
   auto issue = [&](const void* base, int64_t sb, int64_t ss, int64_t sh, int ti, int b, int blk) {
     const int c0 = (t % TPK) * CPT;
@@ -728,7 +729,15 @@ Plan plan_of(const fxpr_attention_params* a) {
   return pl;
 }
 
-attn::Params params_of(const fxpr_attention_params* a, const Plan& pl) {
+// What a call promises about its inputs beyond the unified attention's: rows
+// of q and o that exist, and the extent of the cache that block ids may leave.
+struct Bounds {
+  int64_t tokens;
+  int blocks;
+};
+constexpr Bounds kUnbounded = {INT64_MAX, INT32_MAX};
+
+attn::Params params_of(const fxpr_attention_params* a, const Plan& pl, const Bounds& b) {
   attn::Params p = {};
   p.q = a->q; p.q_dtype = a->q_dtype; p.q_st = a->q_stride_tok; p.q_sh = a->q_stride_head;
   p.k = a->k_cache; p.v = a->v_cache;
@@ -746,6 +755,8 @@ attn::Params params_of(const fxpr_attention_params* a, const Plan& pl) {
   p.exact_qk = (a->q_dtype != FXPR_F32) && (a->kv_dtype != FXPR_F32);
   p.qtiles = pl.qtiles;
   p.one = 1.0f;
+  p.tokens = b.tokens;
+  p.blocks = b.blocks;
   p.page_shift = -1;
   for (int sh = 0; sh < 31; ++sh)
     if ((1 << sh) == a->page_size) p.page_shift = sh;
@@ -854,24 +865,10 @@ int validate_prefix(const fxpr_attention_params* a, int prefix_len, int64_t toke
   return FXPR_OK;
 }
 
-}  // namespace
-
-extern "C" int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* a) {
-  if (validate(a) != FXPR_OK) return 0;
-  if (a->num_requests <= 0 || a->max_query_len <= 0) return 0;
-  return plan_of(a).total;
-}
-
-extern "C" int fxpr_unified_attention_fxp(const fxpr_attention_params* a, void* stream) {
-  const int rc = validate(a);
-  if (rc != FXPR_OK) return rc;
+// the unified kernels on checked parameters of at least one request
+int run_unified(const fxpr_attention_params* a, const Plan& pl, const Bounds& b, cudaStream_t st) {
   const int D = a->head_dim;
-  const int ra = check_alignment(a);
-  if (ra != FXPR_OK) return ra;
-  if (a->num_requests <= 0 || a->max_query_len <= 0) return FXPR_OK;
-  const Plan pl = plan_of(a);
-  attn::Params p = params_of(a, pl);
-  const cudaStream_t st = (cudaStream_t)stream;
+  attn::Params p = params_of(a, pl, b);
   const int R = a->num_requests;
 
   if (a->workspace && pl.total > 0 && a->workspace_bytes >= pl.total) {
@@ -879,7 +876,7 @@ extern "C" int fxpr_unified_attention_fxp(const fxpr_attention_params* a, void* 
       set_error("unified_attention_fxp: workspace must be 256-byte aligned");
       return FXPR_ERR_INVALID;
     }
-    if (pl.decode_kmax > 0) return attn::launch_decode(a, pl.decode_kmax, a->workspace, st);
+    if (pl.decode_kmax > 0) return attn::launch_decode(a, b.tokens, pl.decode_kmax, a->workspace, st);
     unsigned char* ws = reinterpret_cast<unsigned char*>(a->workspace);
     p.ws_cnt = reinterpret_cast<uint32_t*>(ws);
     p.ws_acc = reinterpret_cast<unsigned long long*>(ws + pl.off_acc);
@@ -916,6 +913,22 @@ extern "C" int fxpr_unified_attention_fxp(const fxpr_attention_params* a, void* 
   }
 }
 
+}  // namespace
+
+extern "C" int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* a) {
+  if (validate(a) != FXPR_OK) return 0;
+  if (a->num_requests <= 0 || a->max_query_len <= 0) return 0;
+  return plan_of(a).total;
+}
+
+extern "C" int fxpr_unified_attention_fxp(const fxpr_attention_params* a, void* stream) {
+  int rc = validate(a);
+  if (rc == FXPR_OK) rc = check_alignment(a);
+  if (rc != FXPR_OK) return rc;
+  if (a->num_requests <= 0 || a->max_query_len <= 0) return FXPR_OK;
+  return run_unified(a, plan_of(a), kUnbounded, (cudaStream_t)stream);
+}
+
 extern "C" int64_t fxpr_shared_prefix_attention_workspace_bytes(const fxpr_attention_params* a, int common_prefix_len,
                                                                 int64_t num_tokens) {
   if (validate_prefix(a, common_prefix_len, num_tokens) != FXPR_OK) return 0;
@@ -929,10 +942,12 @@ extern "C" int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* a, 
   int rc = validate_prefix(a, common_prefix_len, num_tokens);
   if (rc != FXPR_OK) return rc;
   if (a->num_requests <= 0 || a->max_query_len <= 0 || num_tokens <= 0) return FXPR_OK;
-  const PrefixPlan pp = prefix_plan_of(a, common_prefix_len, num_tokens);
-  if (!pp.use || a->workspace == nullptr) return fxpr_unified_attention_fxp(a, stream);
   rc = check_alignment(a);
   if (rc != FXPR_OK) return rc;
+  const PrefixPlan pp = prefix_plan_of(a, common_prefix_len, num_tokens);
+  const int64_t nb = a->num_blocks;
+  const Bounds bounds = {num_tokens, (int)(nb < 0 ? 0 : nb < INT32_MAX ? nb : INT32_MAX)};
+  if (!pp.use || a->workspace == nullptr) return run_unified(a, pp.pl, bounds, (cudaStream_t)stream);
   if (a->workspace_bytes < pp.total || (uintptr_t)a->workspace % 256 != 0) {
     set_error("shared_prefix_attention_fxp: the workspace must be 256-byte aligned and hold %lld bytes", (long long)pp.total);
     return FXPR_ERR_INVALID;
@@ -940,7 +955,7 @@ extern "C" int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* a, 
   const Plan& pl = pp.pl;
   const cudaStream_t st = (cudaStream_t)stream;
   unsigned char* ws = reinterpret_cast<unsigned char*>(a->workspace);
-  attn::Params p = params_of(a, pl);
+  attn::Params p = params_of(a, pl, bounds);
   p.ws_cnt = reinterpret_cast<uint32_t*>(ws);
   p.row_max = reinterpret_cast<uint32_t*>(ws + pp.off_max);
   p.row_den = reinterpret_cast<unsigned long long*>(ws + pp.off_den);
@@ -948,7 +963,6 @@ extern "C" int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* a, 
   p.ws_s = reinterpret_cast<float*>(ws + pp.off_s);
   p.nchunk_max = pp.nchunk;
   p.key0 = pp.key0;
-  p.tokens = num_tokens;
   float* scores = reinterpret_cast<float*>(ws + pp.off_p);
   if (cudaMemsetAsync(ws, 0, pp.off_s, st) != cudaSuccess) return check_launch("fxpr_shared_prefix_attention_fxp (clear)");
   rc = attn::launch_suffix(p, false, a->head_dim, pl.rp, a->int_bits, a->kv_dtype, a->num_requests, pl.ys, st);

@@ -87,7 +87,7 @@ __device__ __forceinline__ int unit_rows(const Params& p, int req, int qtile, in
     const int qoff = qtile * p.qt + qi;
     const int hg = hslice * p.gs + gh;
     int tok = -1, kend = 0, pos = 0, head = 0;
-    if (qi < p.qt && qoff < qlen && hg < p.group) {
+    if (qi < p.qt && qoff < qlen && hg < p.group && q_start + qoff < p.tokens) {
       tok = q_start + qoff;
       head = kvh * p.group + hg;
       pos = ctx + qoff;
@@ -122,7 +122,8 @@ struct TileCopier {
     const int j = kb + ti * NK + my_jl;
     if (j >= ke) return -1;
     const int bi = p.page_shift >= 0 ? (j >> p.page_shift) : j / p.page;
-    return p.bt[bt_row + bi];
+    const int b = p.bt[bt_row + bi];
+    return b < p.blocks ? b : -1;
   }
   __device__ __forceinline__ void issue(const void* base, int64_t sb, int64_t ss, int64_t sh,
                                         int ti, unsigned char* dst_tile, int blk) const {
@@ -231,11 +232,7 @@ __global__ void __launch_bounds__(THREADS) chunk_scores_kernel(Params p) {
   if constexpr (PRE) launch_dependents();
   int kr_hi = unit_rows<RP>(p, req, qtile, kvh, hslice, row_tok, row_head, row_pos, row_kend);
   if (kr_hi < 0) return;  // uniform over the CTA
-  if constexpr (PRE) {
-    kr_hi = max(kr_hi, p.key0);
-    if (threadIdx.x < RP && row_tok[threadIdx.x] >= p.tokens) row_tok[threadIdx.x] = -1;  // no such row of q
-    __syncthreads();
-  }
+  if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
   const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
   if (chunk > 0 && kb >= kr_hi) return;
   const int ke = min(kb + CHUNK, kr_hi);
@@ -675,11 +672,7 @@ __global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_ker
     if constexpr (PRE) wait_dependencies();  // the launch ends after the one it overlaps
     return;
   }
-  if constexpr (PRE) {
-    kr_hi = max(kr_hi, p.key0);
-    if (threadIdx.x < RP && row_tok[threadIdx.x] >= p.tokens) row_tok[threadIdx.x] = -1;  // no such row of q
-    __syncthreads();
-  }
+  if constexpr (PRE) kr_hi = max(kr_hi, p.key0);
   const int kb = (PRE ? p.key0 : 0) + chunk * CHUNK;
   if (chunk > 0 && kb >= kr_hi) {
     if constexpr (PRE) wait_dependencies();

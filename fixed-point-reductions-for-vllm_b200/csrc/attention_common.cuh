@@ -46,6 +46,11 @@ struct Params {
   int qtiles;
   int page_shift;  // log2(page) when page is a power of two, else -1
   float one;      // 1.0f, opaque to the compiler (magic add as an FMA)
+  // the shared-prefix operator's bounds (none for the unified attention): rows
+  // of q and o from `tokens` on do not exist, and a block id outside
+  // [0, blocks) reads zeros
+  int64_t tokens;
+  int blocks;
   // chunked path: caller workspace (no state between calls)
   uint32_t* ws_cnt;            // [items] chunks finished
   unsigned long long* ws_acc;  // [items][RP][D] integer PV partial sums
@@ -56,7 +61,6 @@ struct Params {
   // shared-prefix form: keys before key0 belong to the prefix kernels
   // (attention_prefix.cu); rows are token * num_heads + head
   int key0;
-  int64_t tokens;               // rows of q and o
   uint32_t* row_max;            // [rows] row maxima over all keys, as ordered integers
   unsigned long long* row_den;  // [rows] integer normaliser partial sums
   unsigned long long* row_acc;  // [rows][D] integer PV partial sums
@@ -176,7 +180,7 @@ inline int launch_overlapped(void (*kernel)(Arg), dim3 grid, size_t smem, cudaSt
 // decode path for grouped-query batches (attention_decode.cu)
 bool decode_supported(const fxpr_attention_params* a, int G);
 int64_t decode_workspace_bytes(int items, int kmax, int D);
-int launch_decode(const fxpr_attention_params* a, int kmax, void* workspace, cudaStream_t st);
+int launch_decode(const fxpr_attention_params* a, int64_t tokens, int kmax, void* workspace, cudaStream_t st);
 
 // chunked two-kernel path (attention_chunked.cu)
 bool chunked_supported(int D, int rp, int kv_dtype);

@@ -67,6 +67,8 @@ struct DqParams {
   const int32_t* bt;
   int64_t bt_stride;
   int R, KVH, page, page_shift, kmax;
+  int64_t tokens;  // rows of q and o that exist
+  int blocks;      // blocks of the cache
   float scale_log2;
   int frac;
   float one;
@@ -87,13 +89,14 @@ template <int D> struct Geo {
   static constexpr int DPL = D / 32;          // dims per lane (pv)
 };
 
-// pages of every item of request r (0 without a query row); kend = keys
+// pages of every item of request r (0 without a query row, or if that row
+// does not exist); kend = keys
 __device__ __forceinline__ int pages_of(const DqParams& p, int r, int* kend) {
   const int qlen = p.qsl[r + 1] - p.qsl[r];
   const int sl = p.seq_lens[r];
   const int ke = min(sl, p.kmax);
   if (kend) *kend = ke;
-  if (qlen < 1) return 0;
+  if (qlen < 1 || p.qsl[r] >= p.tokens) return 0;
   return max(1, (ke + PG - 1) / PG);
 }
 
@@ -158,7 +161,8 @@ __device__ __forceinline__ Slot resolve(const DqParams& p, const int* pre, int b
     const int col = p.page_shift >= 0 ? (key0 >> p.page_shift) : key0 / p.page;
     const int slot0 = key0 - col * p.page;
     s.kc = kvh | (slot0 << 16);
-    s.blk = __ldg(p.bt + (int64_t)r * p.bt_stride + col);
+    const int b = __ldg(p.bt + (int64_t)r * p.bt_stride + col);
+    s.blk = b < p.blocks ? b : -1;  // a box outside the tensor map reads zeros
   }
   return s;
 }
@@ -854,7 +858,7 @@ bool decode_supported(const fxpr_attention_params* a, int G) {
   return true;
 }
 
-int launch_decode(const fxpr_attention_params* a, int kmax, void* workspace, cudaStream_t st) {
+int launch_decode(const fxpr_attention_params* a, int64_t tokens, int kmax, void* workspace, cudaStream_t st) {
   using namespace dq;
   const int D = a->head_dim;
   const int items = a->num_requests * a->num_kv_heads;
@@ -886,6 +890,8 @@ int launch_decode(const fxpr_attention_params* a, int kmax, void* workspace, cud
   for (int sh = 0; sh < 31; ++sh)
     if ((1 << sh) == a->page_size) p.page_shift = sh;
   p.kmax = kmax;
+  p.tokens = tokens;
+  p.blocks = (int)(a->num_blocks < INT32_MAX ? a->num_blocks : INT32_MAX);
   p.scale_log2 = a->scale_log2;
   p.frac = a->frac_bits;
   p.one = 1.0f;

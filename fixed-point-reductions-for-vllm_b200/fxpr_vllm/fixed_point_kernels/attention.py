@@ -161,7 +161,8 @@ def shared_prefix_attention_fxp(
     finite V the result has the bits of ``unified_attention_fxp``; a masked key
     contributes nothing even where its V is infinite or NaN, and a row which
     sees no key is 0. Rows of ``o`` behind ``query_start_loc[-1]`` are
-    left as they are. ``max_seq_len`` bounds every ``seq_lens`` entry when
+    left as they are, queries behind the rows of ``q`` are skipped, and a block
+    id outside the cache reads zeros. ``max_seq_len`` bounds every ``seq_lens`` entry when
     given, as there. Scratch is a tensor of the call, so calls on several
     streams and captured graphs share nothing."""
     what = "shared_prefix_attention_fxp"

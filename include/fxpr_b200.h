@@ -183,8 +183,8 @@ int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* p);
  * bits of fxpr_unified_attention_fxp; a masked key contributes nothing even
  * where its V is infinite or NaN, and a row that sees no key is 0.
  * num_tokens: rows of q and o; rows behind query_start_loc[num_requests] are
- * left as they are. num_blocks must be given; a prefix block id outside the
- * cache reads zeros. Calls that the prefix kernels do not take (head_dim 32 or
+ * left as they are, and queries behind row num_tokens are skipped. num_blocks
+ * must be given; a block id outside [0, num_blocks) reads zeros. Calls that the prefix kernels do not take (head_dim 32 or
  * 256, a 32-bit type, a short prefix, few rows, no workspace) run the unified
  * kernels. The workspace is 256-byte aligned, any contents. */
 int64_t fxpr_shared_prefix_attention_workspace_bytes(const fxpr_attention_params* p, int common_prefix_len,

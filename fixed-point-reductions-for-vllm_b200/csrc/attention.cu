@@ -435,8 +435,12 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
       float pv = 0.0f;
       if (j < ke) {
         const float sc = recompute ? S_tmp[prow * KT + jl] : S[prow * (p.cap + 8) + ti * KT + jl];
-        pv = prim_exp2(__fsub_rn(sc, gm));
-        if (j < kend_p) den_acc += (UAcc)f2x_f32<BITS>(pv, scale);
+        if (p.skip_masked && sc == -INFINITY) {
+          pv = -0.0f;
+        } else {
+          pv = prim_exp2(__fsub_rn(sc, gm));
+          if (j < kend_p) den_acc += (UAcc)f2x_f32<BITS>(pv, scale);
+        }
       }
       // key slot: the KPT keys of PV thread group kg are contiguous
       P[prow * KT + (jl % KG) * KPT + jl / KG] = __fmul_rn(pv, scale);
@@ -505,6 +509,7 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
         for (int i = 0; i < RP; ++i) {
           if (j >= row_kend[i]) continue;
           const float ps = P[i * KT + kg * KPT + u];
+          if (__float_as_uint(ps) == 0x80000000u) continue;  // masked (exp2 gives no -0)
           const auto x0 = f2x_scaled<BITS>(__fmul_rn(ps, vv.x));
           const auto x1 = f2x_scaled<BITS>(__fmul_rn(ps, vv.y));
           if constexpr (BITS == 64) {
@@ -729,13 +734,16 @@ Plan plan_of(const fxpr_attention_params* a) {
   return pl;
 }
 
-// What a call promises about its inputs beyond the unified attention's: rows
-// of q and o that exist, and the extent of the cache that block ids may leave.
+// What the shared-prefix operator promises beyond the unified attention: rows
+// of q and o that exist, the extent of the cache that block ids may leave, and
+// masked keys without any contribution. (The decode kernels need no flag: there
+// a masked key is one behind the context, which they do not read.)
 struct Bounds {
   int64_t tokens;
   int blocks;
+  int skip_masked;
 };
-constexpr Bounds kUnbounded = {INT64_MAX, INT32_MAX};
+constexpr Bounds kUnbounded = {INT64_MAX, INT32_MAX, 0};
 
 attn::Params params_of(const fxpr_attention_params* a, const Plan& pl, const Bounds& b) {
   attn::Params p = {};
@@ -757,6 +765,7 @@ attn::Params params_of(const fxpr_attention_params* a, const Plan& pl, const Bou
   p.one = 1.0f;
   p.tokens = b.tokens;
   p.blocks = b.blocks;
+  p.skip_masked = b.skip_masked;
   p.page_shift = -1;
   for (int sh = 0; sh < 31; ++sh)
     if ((1 << sh) == a->page_size) p.page_shift = sh;
@@ -946,7 +955,7 @@ extern "C" int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* a, 
   if (rc != FXPR_OK) return rc;
   const PrefixPlan pp = prefix_plan_of(a, common_prefix_len, num_tokens);
   const int64_t nb = a->num_blocks;
-  const Bounds bounds = {num_tokens, (int)(nb < 0 ? 0 : nb < INT32_MAX ? nb : INT32_MAX)};
+  const Bounds bounds = {num_tokens, (int)(nb < 0 ? 0 : nb < INT32_MAX ? nb : INT32_MAX), 1};
   if (!pp.use || a->workspace == nullptr) return run_unified(a, pp.pl, bounds, (cudaStream_t)stream);
   if (a->workspace_bytes < pp.total || (uintptr_t)a->workspace % 256 != 0) {
     set_error("shared_prefix_attention_fxp: the workspace must be 256-byte aligned and hold %lld bytes", (long long)pp.total);

@@ -640,8 +640,7 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
 // kernel 2: normaliser, PV and the integer combine
 // ---------------------------------------------------------------------------
 // PRE: over the keys from p.key0 on; the row maxima are complete, the sums of
-// the keys before are in the row accumulators, and a masked key (score -inf,
-// kept as p = -0) contributes nothing whatever its V holds.
+// the keys before are in the row accumulators.
 template <int D, int RP, int BITS, typename KVT, bool PRE = false>
 __global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_kernel(Params p) {
   constexpr int NBP = PRE ? NBP_PRE : attn::NBP;
@@ -733,7 +732,7 @@ __global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_ker
     const int j = kb + k;
     float pv = 0.0f;
     UAcc den = 0;
-    if (PRE && (j >= ke || P_all[i * CHUNK + k] == -INFINITY)) {
+    if ((PRE || p.skip_masked) && (j >= ke || P_all[i * CHUNK + k] == -INFINITY)) {
       pv = -0.0f;
     } else if (j < ke) {
       pv = prim_exp2(__fsub_rn(P_all[i * CHUNK + k], gmax_s[i]));
@@ -853,7 +852,7 @@ __global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_ker
         for (int i = 0; i < RP; ++i) {
           if (j >= row_kend[i]) continue;
           const float ps = Pk[i * CHUNK + u];
-          if (PRE && __float_as_uint(ps) == 0x80000000u) continue;
+          if (__float_as_uint(ps) == 0x80000000u) continue;  // masked (exp2 gives no -0)
           const auto x0 = f2x_scaled<BITS>(__fmul_rn(ps, vv.x));
           const auto x1 = f2x_scaled<BITS>(__fmul_rn(ps, vv.y));
           if constexpr (BITS == 64) {

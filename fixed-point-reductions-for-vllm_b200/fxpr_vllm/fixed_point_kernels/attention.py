@@ -158,9 +158,9 @@ def shared_prefix_attention_fxp(
     The first ``common_prefix_len // page`` entries of every block-table row
     are the same pages (those of row 0 are read), and the keys of a last page
     that the prefix covers in part are equal in every request's own page. With
-    finite V the result has the bits of ``unified_attention_fxp``; a masked key
-    contributes nothing even where its V is infinite or NaN, and a row which
-    sees no key is 0. Rows of ``o`` behind ``query_start_loc[-1]`` are
+    V finite in fp16 (to which it is cast) the result has the bits of
+    ``unified_attention_fxp``; a masked key contributes nothing whatever its V
+    holds, and a row which sees no key is 0, in every form that a call may run. Rows of ``o`` behind ``query_start_loc[-1]`` are
     left as they are, queries behind the rows of ``q`` are skipped, and a block
     id outside the cache reads zeros. ``max_seq_len`` bounds every ``seq_lens`` entry when
     given, as there. Scratch is a tensor of the call, so calls on several

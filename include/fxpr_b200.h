@@ -179,9 +179,10 @@ int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* p);
  * common_prefix_len keys: the block table rows of all requests start with the
  * same common_prefix_len / page_size pages (row 0's are read) and the keys of
  * a last, partly shared page are equal. The prefix's keys and values are read
- * once for a tile of rows of all requests. With finite V the result has the
- * bits of fxpr_unified_attention_fxp; a masked key contributes nothing even
- * where its V is infinite or NaN, and a row that sees no key is 0.
+ * once for a tile of rows of all requests. With V finite in fp16 (to which it
+ * is cast) the result has the bits of fxpr_unified_attention_fxp; a masked key
+ * contributes nothing whatever its V holds, and a row that sees no key is 0, in
+ * every form that a call may run.
  * num_tokens: rows of q and o; rows behind query_start_loc[num_requests] are
  * left as they are, and queries behind row num_tokens are skipped. num_blocks
  * must be given; a block id outside [0, num_blocks) reads zeros. Calls that the prefix kernels do not take (head_dim 32 or

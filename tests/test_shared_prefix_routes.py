@@ -72,3 +72,67 @@ def test_queries_behind_the_rows_are_skipped(route):
     guard = torch.full((q.shape[0] + 8, *q.shape[1:]), 7.0, device="cuda")
     A.shared_prefix_attention_fxp(q[:n], kv, guard[:n], qsl, sl, bt, prefix, mq, max_seq_len=ms)
     assert bits_equal(guard[:n], want[:n]) and (guard[n:] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 64])
+@pytest.mark.parametrize("route", ROUTES)
+def test_masked_keys_contribute_nothing(route, bits):
+    """V of keys that a row does not see may be infinite or NaN: a window's hidden pages, later queries' keys, places behind the end."""
+    batch = _batch(route)
+    (q, kv, qsl, sl, bt), prefix, mq, _ = batch
+    want = _run(batch, fxp_dtype=bits)
+    for r, n in enumerate(sl.tolist()):  # behind the sequence's end, on its last page
+        kv[bt[r, n // PAGE].long(), 1, n % PAGE:] = float("nan")
+    assert bits_equal(_run(batch, fxp_dtype=bits), want)
+    if mq > 1:  # the last query's own key, hidden from the queries before it
+        r = int(torch.argmax(qsl[1:] - qsl[:-1]))
+        j = int(sl[r]) - 1
+        kv[bt[r, j // PAGE].long(), 1, j % PAGE] = float("inf")
+        got, last = _run(batch, fxp_dtype=bits), int(qsl[r + 1]) - 1
+        keep = [t for t in range(q.shape[0]) if t != last]
+        assert bits_equal(got[keep], want[keep])
+        return
+    want = _run(batch, fxp_dtype=bits, window_size=64)
+    kv[bt[0, :prefix // PAGE - 5].long(), 1] = float("inf")
+    kv[bt[0, 2].long(), 1] = float("nan")
+    assert bits_equal(_run(batch, fxp_dtype=bits, window_size=64), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 64])
+@pytest.mark.parametrize("route", ROUTES)
+def test_rows_that_see_no_key_are_zero(route, bits):
+    """A request without keys, and queries in front of a sequence shorter than their number."""
+    batch = _batch(route)
+    (q, _, qsl, sl, _), _, mq, _ = batch
+    want = _run(batch, fxp_dtype=bits)
+    sl[0] = 0
+    blind = [0]
+    if mq > 1:
+        sl[3] = 1  # four queries, one key: three rows see nothing
+        blind += list(range(int(qsl[3]), int(qsl[4]) - 1))
+    got = _run(batch, fxp_dtype=bits)
+    assert (got[blind] == 0).all() and got.isfinite().all()
+    rest = list(range(int(qsl[1]), int(qsl[3])))
+    assert bits_equal(got[rest], want[rest])
+    window = _run(batch, fxp_dtype=bits, window_size=64)
+    assert (window[blind] == 0).all()
+
+
+@pytest.mark.gpu
+def test_a_request_does_not_see_its_batch():
+    """Requests with infinite V behind a window, one of them without keys: the same bits by the unified kernels as by the prefix
+    kernels."""
+    batch = _batch("chunks, one query")
+    (q, kv, qsl, sl, bt), prefix, mq, ms = batch
+    kv[bt[0, :3].long(), 1] = float("inf")
+    sl[2] = 0
+    small = _run(batch, window_size=64)
+    # the same requests behind 128 more keys that their window hides: from 256 shared keys on the prefix kernels run
+    extra = torch.randn(8, *kv.shape[1:], device="cuda").to(kv.dtype)
+    extra[:, 1] = float("nan")
+    more = torch.cat([(kv.shape[0] + torch.arange(8, device="cuda").int()).expand(4, -1), bt], 1)
+    far = torch.where(sl > 0, sl + 128, 0).int()
+    large = _run(((q, torch.cat([kv, extra]), qsl, far, more), prefix + 128, mq, ms + 128), window_size=64)
+    assert bits_equal(small, large)

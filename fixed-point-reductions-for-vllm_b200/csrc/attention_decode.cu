@@ -161,8 +161,7 @@ __device__ __forceinline__ Slot resolve(const DqParams& p, const int* pre, int b
     const int col = p.page_shift >= 0 ? (key0 >> p.page_shift) : key0 / p.page;
     const int slot0 = key0 - col * p.page;
     s.kc = kvh | (slot0 << 16);
-    const int b = __ldg(p.bt + (int64_t)r * p.bt_stride + col);
-    s.blk = b < p.blocks ? b : -1;  // a box outside the tensor map reads zeros
+    s.blk = __ldg(p.bt + (int64_t)r * p.bt_stride + col);
   }
   return s;
 }
@@ -276,11 +275,13 @@ struct Pipe {
   __device__ __forceinline__ int2 item_pg(int i) const {
     return make_int2(__shfl_sync(0xffffffffu, A.item, i & 31), __shfl_sync(0xffffffffu, A.pg, i & 31));
   }
-  // coordinates of page i: (kv head | slot0 << 16, block)
-  __device__ __forceinline__ int2 coords(int i) const {
+  // coordinates of page i: (kv head | slot0 << 16, block), with an id behind
+  // the cache as -1 (a box outside the tensor map reads zeros). Checked here,
+  // not in resolve(): there it would wait for the block-table read.
+  __device__ __forceinline__ int2 coords(const DqParams& p, int i) const {
     const bool b = (i >> 5) != a_idx;
-    return make_int2(__shfl_sync(0xffffffffu, b ? B.kc : A.kc, i & 31),
-                     __shfl_sync(0xffffffffu, b ? B.blk : A.blk, i & 31));
+    const int blk = __shfl_sync(0xffffffffu, b ? B.blk : A.blk, i & 31);
+    return make_int2(__shfl_sync(0xffffffffu, b ? B.kc : A.kc, i & 31), blk < p.blocks ? blk : -1);
   }
 };
 
@@ -355,7 +356,7 @@ dq_scores_kernel(const __grid_constant__ CUtensorMap kmap, const DqParams p) {
   pp.B = resolve(p, pre, G0 + 32, G1);
   pp.a_idx = 0;
   auto issue = [&](int i) {
-    const int2 c = pp.coords(i);
+    const int2 c = pp.coords(p, i);
     if (lane == 0) {
       uint64_t* bar = &bars[i % S];
       tma::fence_proxy_async();
@@ -586,7 +587,7 @@ dq_pv_kernel(const __grid_constant__ CUtensorMap vmap, const DqParams p) {
   pp.B = resolve(p, pre, G0 + 32, G1);
   pp.a_idx = 0;
   auto issue = [&](int i) {
-    const int2 c = pp.coords(i);
+    const int2 c = pp.coords(p, i);
     if (lane == 0) {
       uint64_t* bar = &bars[i % S];
       unsigned char* dst = stage0 + (i % S) * STB;

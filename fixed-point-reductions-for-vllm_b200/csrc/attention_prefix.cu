@@ -21,7 +21,7 @@
 // Bound: the FMA and integer pipes. Each of the 2 * head_dim products per
 // (row, key) is rounded to the 2^-f grid by itself (FFMA2 + IADD3 a pair in
 // q.k; FMUL2 + FFMA2 + IADD3 in p.v, whose product is not exact), which a
-// tensor core cannot do. What the shared rows buy is that the other
+// tensor core cannot do. (Twice that where values are too large for it, below.) What the shared rows buy is that the other
 // instructions go away: a thread holds 8 rows x 2 keys (or 4 dims), so an
 // operand from shared memory feeds up to 8 products and the conversion of K
 // and V is shared by the 64 rows of the tile.
@@ -122,6 +122,38 @@ template <typename T> __device__ __forceinline__ float2 pair_of(uint32_t w) {
   }
 }
 
+// Rounding a product x to the 2^-f grid, by how large the products of a block
+// can be (max|a| * max|b| * 2^f, strict):
+//   fast  below 2^22: one addition of the magic constant
+//   wide  below LIMIT: first to multiples of 2^U (a constant 2^U times larger),
+//         then the rest, x - h * 2^U, with the constant again; both are exact
+//         but for the one rounding at the end, so h * 2^U + l = RNE(x). Three
+//         packed operations and two integer additions a pair instead of one
+//         and one; sums of h and of l stay in 32 bits.
+//   else  the definition's clamp and convert (saturation, infinities, NaN)
+// An outlier channel, a request of large queries and grids finer than 2^-18
+// leave the fast range, and are common. 64 requests behind 4096 keys, 32 / 8
+// heads x 128, bf16, 32 bits, the whole operator (unified attention): ordinary
+// values 237 us (283), a 20-fold channel of K 274 us (783), one request's
+// queries 20-fold 283 us (523), a 60-fold channel of V 377 us (584), 20
+// fraction bits 466 us (848), 24 bits 514 us (1105). 30 bits, where nearly all
+// products saturate, 1186 us (1108).
+template <int BITS> struct Wide {
+  static constexpr int U = BITS == 64 ? 20 : 10;
+  static constexpr float LIMIT = BITS == 64 ? 4398046511104.0f : 2147483136.0f;  // 2^42; 2^31 - 2^9: no saturation
+  static constexpr float C = BITS == 64 ? 13194139533312.0f : 12884901888.0f;    // 1.5 * 2^(23 + U)
+  static constexpr uint32_t CBITS = (uint32_t)(150 + U) << 23 | 0x400000u;
+  static constexpr float K = C + kMagic;
+};
+// h and l of two products x (their sums of bit patterns, biased by CBITS and
+// kMagicBits a product). X: x of the pair plus an addend, rounded once.
+template <int BITS, typename X> __device__ __forceinline__ void wide_pair(X x, float2 minus, uint32_t& h, uint32_t& l) {
+  const float2 r = x(make_float2(Wide<BITS>::C, Wide<BITS>::C));
+  const float2 s = x(fma2(r, minus, make_float2(Wide<BITS>::K, Wide<BITS>::K)));
+  h += __float_as_uint(r.x) + __float_as_uint(r.y);
+  l += __float_as_uint(s.x) + __float_as_uint(s.y);
+}
+
 // element offset of key j, on block blk, from its KV head's first key
 __device__ __forceinline__ int64_t key_offset(const Params& p, int j, int blk, int sb, int ss) {
   const int slot = p.page_shift >= 0 ? (j & (p.page - 1)) : j % p.page;
@@ -154,22 +186,29 @@ struct ScoresSmem {
 // head_dim 64.
 constexpr int SCORES_CTAS = 2;
 constexpr int SU = 4;
+constexpr int BD = 16;  // dims of a block that is rounded one way
 
 template <int D, int RT, int BITS, typename T, bool PL>
 __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(const __grid_constant__ Args a) {
   constexpr int TM = RT / 8, TN = KT64 / 32, NCH = D / DC;
-  constexpr int Q_LD = ScoresSmem<D, RT>::Q_LD;
+  using SM = ScoresSmem<D, RT>;
+  using W = Wide<BITS>;
+  using UAcc = typename std::conditional<BITS == 64, unsigned long long, uint32_t>::type;
+  constexpr int Q_LD = SM::Q_LD;
   constexpr int LOADS = KT64 * DC / 8 / THREADS;  // 16-byte loads of K per thread and step
   const Params& p = a.p;
   extern __shared__ __align__(16) unsigned char smem[];
   float* q_s = reinterpret_cast<float*>(smem);
-  float* k_s = reinterpret_cast<float*>(smem + ScoresSmem<D, RT>::off_k);
+  float* k_s = reinterpret_cast<float*>(smem + SM::off_k);
   __shared__ Rows<RT> rows;
-  __shared__ uint32_t q_max, k_max[3];
+  __shared__ uint32_t q_max;
 
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const float scale = ldexpf(1.0f, p.frac);
-  const float2 C2 = make_float2(kMagic, kMagic);
+  const float scale = ldexpf(1.0f, p.frac), inv_scale = ldexpf(1.0f, -p.frac);
+  const float2 C2 = make_float2(kMagic, kMagic), MINUS2 = make_float2(-p.one, -p.one);
+  // 64 bits: what the tile's dots have beyond their 32-bit sums, once a block
+  // was not fast; in local memory (volatile), for it is rarely touched
+  volatile unsigned long long rest[BITS == 64 ? TM * TN : 1];
   // K staging: thread t moves 8 dims of key rows t / 8 + 32 * u of a tile
   const int krow = t / (DC / 8), kcol = (t % (DC / 8)) * 8;
   int64_t u0 = a.units * blockIdx.x / gridDim.x;
@@ -183,7 +222,6 @@ __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(con
     u0 += n;
     const int kvh = combo / a.tiles, tile = combo % a.tiles;
     if (t == 0) q_max = 0u;
-    if (t < 3) k_max[t] = 0u;
     tile_rows<RT>(a, a.tile0 + tile, kvh, rows);
     {
       uint32_t qo = 0;
@@ -245,7 +283,7 @@ __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(con
         if (at[u] >= 0) raw[u] = *reinterpret_cast<const uint4*>(khead + kcol + at[u] + ch * DC);
       }
     };
-    auto store = [&](int it) {
+    auto store = [&](int it) -> float {  // returns the largest |k| that this thread staged
       float* dst = k_s + (it & 1) * KT64 * K_LD;
       uint32_t m = 0;
 #pragma unroll
@@ -259,17 +297,17 @@ __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(con
         *reinterpret_cast<float4*>(d) = make_float4(f0.x, f0.y, f1.x, f1.y);
         *reinterpret_cast<float4*>(d + 4) = make_float4(f2.x, f2.y, f3.x, f3.y);
       }
-      const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax_value<T>(m)));
-      if (lane == 0) atomicMax(&k_max[(it / NCH) % 3], b);
+      return absmax_value<T>(m);
     };
     addresses(0, at_next);
     load(0);
-    store(0);
+    const float first = store(0);
     if (steps > 1) load(1);
     __syncthreads();
-    // max|q| * max|k| * 2^f < 2^22: no saturation, and the magic constant rounds every product exactly
+    // max|q| * max|k| * 2^f < 2^22 over the tile's rows and a step's keys: the fast rounding
     const double scale_d = ldexp(1.0, p.frac), mq = (double)__uint_as_float(q_max);
     const float kthr = mq * scale_d < 3.0e38 ? __double2float_rd(4194304.0 / (mq * scale_d)) : 0.0f;
+    bool large = __syncthreads_or(!(first < kthr));  // of the step to come, uniform over the CTA
 
     float rmax[TM];
     uint32_t acc[TM][TN];
@@ -277,6 +315,7 @@ __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(con
     for (int i = 0; i < TM; ++i) rmax[i] = -INFINITY;
     float* out = a.scores + (((int64_t)kvh * a.tiles + tile) * RT + warp * TM) * p.key0 + kt0 * KT64 + lane;
 
+    bool high = false;  // 64 bits: the tile's dots have a part in `rest` (uniform over the warp)
     for (int it = 0; it < steps; ++it) {
       const int ti = it / NCH, ch = it % NCH;
       if (ch == 0) {
@@ -284,12 +323,11 @@ __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(con
         for (int i = 0; i < TM; ++i)
 #pragma unroll
           for (int j = 0; j < TN; ++j) acc[i][j] = 0u - (uint32_t)D * (uint32_t)kMagicBits;
-        if (t == 0) k_max[(ti + 2) % 3] = 0u;  // read in the tile before; staged again after the next barrier
+        high = false;
       }
       const float* qb = q_s + warp * TM * Q_LD + ch * DC;
       const float* kb_s = k_s + (it & 1) * KT64 * K_LD + lane * K_LD;
-#pragma unroll SU
-      for (int kk = 0; kk < DC; kk += 4) {
+      auto fast4 = [&](int kk) {  // dims kk .. kk + 3
         float4 kv[TN];
 #pragma unroll
         for (int j = 0; j < TN; ++j) kv[j] = *reinterpret_cast<const float4*>(kb_s + j * 32 * K_LD + kk);
@@ -305,33 +343,111 @@ __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(con
             acc[i][j] += __float_as_uint(r1.x) + __float_as_uint(r1.y);
           }
         }
-      }
-      if (ch == NCH - 1) {  // the tile's dots are complete: scores, row maxima
-        const bool fast = __uint_as_float(k_max[ti % 3]) < kthr;  // uniform over the CTA
-        if (!fast) {
-          // values the constant cannot round: the definition's clamp and convert, from the cache
+      };
+      if (!large) {
+#pragma unroll SU
+        for (int kk = 0; kk < DC; kk += 4) fast4(kk);
+      } else {
+        // by blocks of BD dims and the warp's own rows, so that an outlier
+        // channel, or a request of large queries, costs its own blocks only
 #pragma unroll 1
-          for (int e = 0; e < TM * TN; ++e) {
-            const int r = warp * TM + e / TN, key = (kt0 + ti) * KT64 + lane + 32 * (e % TN);
-            const int kblk = block_of(a, key);
-            typename std::conditional<BITS == 64, unsigned long long, uint32_t>::type s = 0;
-            if (rows.tok[r] >= 0 && kblk >= 0) {
-              const T* kr = khead + key_offset(p, key, kblk, a.k_sb, a.k_ss);
-              const int64_t qo = (int64_t)rows.tok[r] * p.q_st + (int64_t)rows.head[r] * p.q_sh;
-              for (int d = 0; d < D; ++d)
-                s += (decltype(s))f2x_f32<BITS>(__fmul_rn(load_f32(p.q, p.q_dtype, qo + d), to_f32(kr[d])), scale);
-            }
-            const float f = BITS == 64 ? __ll2float_rn((long long)s) : __int2float_rn((int32_t)s);
+        for (int b = 0; b < DC; b += BD) {
+          uint32_t qm = 0, km = 0;
+          auto amax = [](uint32_t& m, const float* src) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            m = max(m, max(max(v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu), max(v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu)));
+          };
+          if (lane < TM * (BD / 4)) amax(qm, qb + lane / (BD / 4) * Q_LD + b + lane % (BD / 4) * 4);
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int kk = 0; kk < BD; kk += 4) amax(km, kb_s + j * 32 * K_LD + b + kk);
+          // q is scaled by 2^f; NaN, and infinity times zero, fail both comparisons
+          const float bound = __fmul_ru(__uint_as_float(__reduce_max_sync(0xffffffffu, qm)),
+                                        __uint_as_float(__reduce_max_sync(0xffffffffu, km)));
+          if (bound < 4194304.0f) {
+#pragma unroll 1
+            for (int kk = b; kk < b + BD; kk += 4) fast4(kk);
+            continue;
+          }
+          auto beyond = [&](int i, int j, unsigned long long v) {  // 64 bits: the part that acc does not hold
+            rest[i * TN + j] = high ? rest[i * TN + j] + v : v;
+          };
+          if (bound < W::LIMIT) {
+            uint32_t h[TM][TN];
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-              for (int j = 0; j < TN; ++j)
-                if (e == i * TN + j) acc[i][j] = __float_as_uint(f);  // kept as its fp32 value
+              for (int j = 0; j < TN; ++j) h[i][j] = 0u - (uint32_t)BD * W::CBITS;
+#pragma unroll 1
+            for (int kk = b; kk < b + BD; kk += 4) {
+              float4 kv[TN];
+#pragma unroll
+              for (int j = 0; j < TN; ++j) kv[j] = *reinterpret_cast<const float4*>(kb_s + j * 32 * K_LD + kk);
+#pragma unroll
+              for (int i = 0; i < TM; ++i) {
+                const float4 qv = *reinterpret_cast<const float4*>(qb + i * Q_LD + kk);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                  wide_pair<BITS>([&](float2 c) { return fma2(make_float2(qv.x, qv.y), make_float2(kv[j].x, kv[j].y), c); },
+                                  MINUS2, h[i][j], acc[i][j]);
+                  wide_pair<BITS>([&](float2 c) { return fma2(make_float2(qv.z, qv.w), make_float2(kv[j].z, kv[j].w), c); },
+                                  MINUS2, h[i][j], acc[i][j]);
+                }
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int j = 0; j < TN; ++j) {
+                if constexpr (BITS == 64) beyond(i, j, (unsigned long long)(long long)(int32_t)h[i][j] << W::U);
+                else acc[i][j] += h[i][j] << W::U;
+              }
+          } else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+              UAcc s[TN] = {};
+#pragma unroll 1
+              for (int kk = b; kk < b + BD; kk += 4) {
+                float kv[TN][4];
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                  *reinterpret_cast<float4*>(kv[j]) = *reinterpret_cast<const float4*>(kb_s + j * 32 * K_LD + kk);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float x = qb[i * Q_LD + kk + e];
+                  float qv = __fmul_rn(x, inv_scale);  // q again, unless its scaling left the fp32 range
+                  if (fabsf(x) == INFINITY) {
+                    const int r = warp * TM + i;
+                    qv = load_f32(p.q, p.q_dtype, (int64_t)rows.tok[r] * p.q_st + (int64_t)rows.head[r] * p.q_sh + ch * DC + kk + e);
+                  }
+#pragma unroll
+                  for (int j = 0; j < TN; ++j) s[j] += (UAcc)f2x_f32<BITS>(__fmul_rn(qv, kv[j][e]), scale);
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < TN; ++j) {
+                acc[i][j] += (uint32_t)BD * (uint32_t)kMagicBits;
+                if constexpr (BITS == 64) beyond(i, j, s[j]);
+                else acc[i][j] += s[j];
+              }
+            }
           }
+          if constexpr (BITS == 64) high = true;
         }
+      }
+      if (ch == NCH - 1) {  // the tile's dots are complete: scores, row maxima
+        if (BITS == 64 && high) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)  // kept as its fp32 value
+              acc[i][j] = __float_as_uint(__ll2float_rn((long long)(int32_t)acc[i][j] + (long long)rest[i * TN + j]));
+        }
+        const bool ints = !(BITS == 64 && high);
         float* dst = out + ti * KT64;
         const int key0 = (kt0 + ti) * KT64;
-        if (PL && fast && key0 >= rows.all_low && key0 + KT64 <= rows.all_high) {  // the usual tile: every row sees every key
+        if (PL && ints && key0 >= rows.all_low && key0 + KT64 <= rows.all_high) {  // the usual tile: every row sees every key
 #pragma unroll
           for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -349,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(con
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
               const int key = key0 + lane + 32 * j;
-              float qk = __fmul_rn(fast ? __int2float_rn((int32_t)acc[i][j]) : __uint_as_float(acc[i][j]), a.score_mul);
+              float qk = __fmul_rn(ints ? __int2float_rn((int32_t)acc[i][j]) : __uint_as_float(acc[i][j]), a.score_mul);
               if constexpr (!PL) {
                 if (p.softcap_log2 > 0.0f) qk = __fmul_rn(p.softcap_log2, prim_tanh(__fmul_rn(qk, p.softcap_rcp)));
                 if (p.alibi) qk = __fmaf_rn(p.alibi[rows.head[r]], __fsub_rn((float)key, (float)rows.pos[r]), qk);
@@ -362,9 +478,10 @@ __global__ void __launch_bounds__(THREADS, SCORES_CTAS) prefix_scores_kernel(con
           }
         }
       }
-      if (it + 1 < steps) store(it + 1);
+      float staged = 0.0f;
+      if (it + 1 < steps) staged = store(it + 1);
       if (it + 2 < steps) load(it + 2);
-      __syncthreads();
+      large = __syncthreads_or(!(staged < kthr) && it + 1 < steps);
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
@@ -405,6 +522,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
   constexpr int VU = (KT64 / 2) * (D / 8) / THREADS;  // (key pair, 8 dims) units per thread
   static_assert(TM >= 1 && SV >= 1 && VU >= 1, "tile mapping");
   using SM = PvSmem<D, RT>;
+  using W = Wide<BITS>;
   const Params& p = a.p;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Rows<RT> rows;
@@ -415,7 +533,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
   // max|v| <= 65504 (finite after the cast) and max|v| * (1 + 2^-10) * 2^f < 2^22, with p <= 1
   const double scale_d = ldexp(1.0, p.frac);
   const float vthr = __double2float_rd(fmin(65504.5, 4194304.0 / (scale_d * (1.0 + 1.0 / 1024))));
-  const float2 C2 = make_float2(kMagic, kMagic), ONE2 = make_float2(p.one, p.one);
+  const float2 C2 = make_float2(kMagic, kMagic), ONE2 = make_float2(p.one, p.one), MINUS2 = make_float2(-p.one, -p.one);
   const bool small_frac = p.frac <= 22;  // p * 2^f <= 2^22: the magic constant rounds it
   const int prow = t / TPR;             // p phase: this row, keys 4 * (t % TPR) + 4 * TPR * u
   const int dl = t % LD, grp = t / LD;  // this thread's dims 4 * dl.., rows grp * TM..
@@ -516,8 +634,8 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][e] = 0u;
-    auto flush = [&](int fast_tiles) {
-      const uint32_t bias = (uint32_t)fast_tiles * (uint32_t)KT64 * (uint32_t)kMagicBits;
+    uint32_t bias = 0;  // of the tiles since the last flush
+    auto flush = [&]() {
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int r = grp * TM + i;
@@ -535,6 +653,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
           acc[i][e] = 0u;
         }
       }
+      bias = 0u;
     };
 
     addresses(0);
@@ -549,13 +668,12 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
       load_v(1);
     }
     __syncthreads();
-    int fast_tiles = 0;
     for (int ti = 0; ti < n; ++ti) {
-      const bool fast = __uint_as_float(v_max[ti % 3]) < vthr;  // uniform over the CTA
+      const float vm = __uint_as_float(v_max[ti % 3]);  // uniform over the CTA
       if (t == 0) v_max[(ti + 2) % 3] = 0u;
       const float* pb = reinterpret_cast<const float*>(smem + SM::off_p + (ti & 1) * SM::p_buf) + grp * TM * P_LD;
       const unsigned char* vs = smem + (ti & 1) * SM::v_buf;
-      if (fast) {
+      if (vm < vthr) {
 #pragma unroll VU_UNROLL
         for (int k = 0; k < KT64; k += 4) {
           float4 w[2][2];  // pairs k/2 and k/2 + 1, dims (0, 1) and (2, 3)
@@ -579,28 +697,86 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
               }
           }
         }
-        ++fast_tiles;
-      } else {  // values the constant cannot round: the definition's clamp and convert
+        bias += (uint32_t)KT64 * (uint32_t)kMagicBits;
+      } else if (vm < __double2float_rd(fmin(65504.5, (double)W::LIMIT / (scale_d * (1.0 + 1.0 / 1024))))) {
+        // 32 bits: h * 2^U + l into the sums. 64 bits: l into the sums, h (zero
+        // for most) to the row's accumulators, RW rows at a time.
+        constexpr int RW = BITS == 32 ? TM : TM < 2 ? 1 : 2;
+#pragma unroll
+        for (int ig = 0; ig < TM; ig += RW) {
+          uint32_t h[RW][4];
+#pragma unroll
+          for (int i = 0; i < RW; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[i][e] = 0u;
 #pragma unroll 1
+          for (int k = 0; k < KT64; k += 2) {
+            const float4 w[2] = {*reinterpret_cast<const float4*>(vs + (size_t)(k / 2) * D * 8 + v0),
+                                 *reinterpret_cast<const float4*>(vs + (size_t)(k / 2) * D * 8 + v1)};
+#pragma unroll
+            for (int i = 0; i < RW; ++i) {
+              const float2 pp = *reinterpret_cast<const float2*>(pb + (ig + i) * P_LD + k);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float4 v = w[e / 2];
+                const float2 x = mul2(pp, e % 2 ? make_float2(v.z, v.w) : make_float2(v.x, v.y));
+                uint32_t hs = 0;
+                wide_pair<BITS>([&](float2 c) { return fma2(x, ONE2, c); }, MINUS2, hs, acc[ig + i][e]);
+                if constexpr (BITS == 32) acc[i][e] += hs << W::U;
+                else h[i][e] += hs;
+              }
+            }
+          }
+          if constexpr (BITS == 64) {
+#pragma unroll
+            for (int i = 0; i < RW; ++i) {
+              const int r = grp * TM + ig + i;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int32_t hv = (int32_t)(h[i][e] - (uint32_t)KT64 * W::CBITS);
+                if (hv && rows.tok[r] >= 0)
+                  atomicAdd(p.row_acc + ((int64_t)rows.tok[r] * p.num_heads + rows.head[r]) * D + 4 * dl + e,
+                            (unsigned long long)(long long)hv << W::U);
+              }
+            }
+          }
+        }
+        bias += (uint32_t)KT64 * ((uint32_t)kMagicBits + (BITS == 32 ? W::CBITS << W::U : 0u));
+      } else {  // the definition's clamp and convert
+#pragma unroll
         for (int i = 0; i < TM; ++i) {
           const int r = grp * TM + i;
-          if (rows.tok[r] < 0) continue;
+          UAcc s[4] = {};
 #pragma unroll 1
-          for (int e = 0; e < 4; ++e) {
-            UAcc s = 0;
-            for (int k = 0; k < KT64; ++k) {
-              const float ps = pb[i * P_LD + k];
-              if (__float_as_uint(ps) == 0x80000000u) continue;
-              const float vv = reinterpret_cast<const float*>(vs + (size_t)(k / 2) * D * 8 + (e < 2 ? v0 : v1))[2 * (e & 1) + (k & 1)];
-              s += (UAcc)f2x_scaled<BITS>(__fmul_rn(ps, vv));
+          for (int k = 0; k < KT64; k += 2) {
+            const float2 pp = *reinterpret_cast<const float2*>(pb + i * P_LD + k);
+            const float4 va4 = *reinterpret_cast<const float4*>(vs + (size_t)(k / 2) * D * 8 + v0);
+            const float4 vb4 = *reinterpret_cast<const float4*>(vs + (size_t)(k / 2) * D * 8 + v1);
+            if (__float_as_uint(pp.x) != 0x80000000u) {  // not masked
+              s[0] += (UAcc)f2x_scaled<BITS>(__fmul_rn(pp.x, va4.x));
+              s[1] += (UAcc)f2x_scaled<BITS>(__fmul_rn(pp.x, va4.z));
+              s[2] += (UAcc)f2x_scaled<BITS>(__fmul_rn(pp.x, vb4.x));
+              s[3] += (UAcc)f2x_scaled<BITS>(__fmul_rn(pp.x, vb4.z));
             }
-            if (s) atomicAdd(p.row_acc + ((int64_t)rows.tok[r] * p.num_heads + rows.head[r]) * D + 4 * dl + e, (unsigned long long)s);
+            if (__float_as_uint(pp.y) != 0x80000000u) {
+              s[0] += (UAcc)f2x_scaled<BITS>(__fmul_rn(pp.y, va4.y));
+              s[1] += (UAcc)f2x_scaled<BITS>(__fmul_rn(pp.y, va4.w));
+              s[2] += (UAcc)f2x_scaled<BITS>(__fmul_rn(pp.y, vb4.y));
+              s[3] += (UAcc)f2x_scaled<BITS>(__fmul_rn(pp.y, vb4.w));
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (BITS == 32) {
+              acc[i][e] += s[e];
+            } else if (s[e] && rows.tok[r] >= 0) {
+              atomicAdd(p.row_acc + ((int64_t)rows.tok[r] * p.num_heads + rows.head[r]) * D + 4 * dl + e, s[e]);
+            }
           }
         }
       }
       if (BITS == 64 && (ti + 1) % RUN == 0) {
-        flush(fast_tiles);
-        fast_tiles = 0;
+        flush();
       }
       if (ti + 1 < n) store(ti + 1);
       if (ti + 2 < n) {
@@ -609,7 +785,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_pv_kernel(const __grid_cons
       }
       __syncthreads();
     }
-    flush(fast_tiles);
+    flush();
 #pragma unroll
     for (int o = 1; o < TPR; o <<= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
     if (t % TPR == 0 && live && den) atomicAdd(p.row_den + row_id, (unsigned long long)den);

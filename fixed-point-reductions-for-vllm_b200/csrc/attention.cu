@@ -788,16 +788,6 @@ int check_alignment(const fxpr_attention_params* a) {
 // ---------------------------------------------------------------------------
 // shared prefix: which calls take the prefix kernels, and their workspace
 // ---------------------------------------------------------------------------
-// Device time of the unified attention over the prefix kernels' (graph
-// replays, 16-bit, 32 query heads unless said):
-//   where it runs its chunk kernels (several queries a request, groups other
-//   than 4, odd pages): prefix of 128 keys 0.6 to 1.35, 512 keys 1.1 to 3.0,
-//   2048 keys 1.4 to 5.7; taken from 256 keys on;
-//   where it runs its decode kernels, (row, key) pairs of the prefix 1 M: 0.9
-//   to 1.05, 4 M: 1.08 (head_dim 128) and 1.27 (64), 8 M: 1.2; fewer launches
-//   make it the faster one for small batches. Taken from 2 M pairs on.
-constexpr int kPrefixMinKeys = 256;
-constexpr int64_t kPrefixMinDecodePairs = 2ll << 20;
 constexpr int64_t kPrefixScores = 128ll << 20;  // about the L2
 
 // Rows per tile: the least total of tiles times a tile's cost, 0.6 : 1 : 1.95
@@ -811,6 +801,50 @@ int prefix_row_tile(int64_t rows) {
   if (cdiv(rows, 32) * 100 < least) best = 32, least = cdiv(rows, 32) * 100;
   if (cdiv(rows, 16) * 60 < least) best = 16;
   return best;
+}
+
+// Whether the prefix kernels are the faster form. Device time of the unified
+// attention over theirs (above 1: they win), 3863 shapes, graph replays, bf16,
+// uniform requests; "own" are the keys behind the prefix.
+//
+// Where the unified attention runs its decode kernels (one query a request,
+// groups of four), own keys run about half as fast here as there, so the
+// prefix has to make up for them: 64 requests, 32 / 8 heads x 128 (x 64)
+//   prefix 4096: own 64 1.28 (1.52), 256 1.17 (1.41), 1024 1.00 (1.16), 8192 0.67 (0.78)
+//   prefix 1024: own 64 0.96 (1.12), 256 0.85 (1.03), 1024 0.70 (0.80), 8192 0.57 (0.66)
+// Taken from 1.9 M (row, key) pairs of prefix on, plus three for each own pair:
+// one of 1008 shapes is then slower, by 2%. And not where most products
+// saturate: 64 requests behind 4096 keys, 28 fraction bits in 32-bit
+// accumulators 907 us against 1109, 30 bits 1186 against 1108; 38 bits in 64-bit
+// accumulators 941 against 1144, 40 bits 1262.
+//
+// Where it runs its chunk kernels, own keys cost the same in both forms, but
+// four launches wait for one another here instead of two. That shows while the
+// unified attention's units (512 keys of an item) do not fill the GPU: 8 / 8
+// heads behind 8192 keys, one request, own 16 0.64, 1024 0.41; four requests
+// 2.03, 1.32; 16 requests 6.7, 3.8; 64 / 8 heads behind 1024 keys, one request,
+// own 64 2.4, 1024 0.9. Hence taken with up to 256 own keys, if a tile has rows
+// to share K with (four a KV head) or the prefix kernels' units are resident at
+// once; and with more where those units exceed 1 wave of CTAs (16-row units), 2
+// (4-row units), 3 (below 8 rows a KV head) or 5 (below 4). Not below 512 prefix
+// keys with many rows and half a wave to a wave of units (0.75 to 1), nor with
+// own keys more than four times the prefix up to 3 waves (0.8 to 1). 57 of 2855
+// shapes are then slower by more than 2%, the worst that several requests can
+// have by 21% (28.5 against 23.5 us); no shape loses more than 1.37 by the rule.
+constexpr int kPrefixMinKeys = 256;
+bool prefix_pays(const fxpr_attention_params* a, const Plan& pl, int key0, int row_tile, int64_t rows_kv) {
+  const int64_t own = pl.max_keys - key0, kv = a->num_kv_heads;
+  if (key0 < kPrefixMinKeys) return false;
+  if (pl.decode_kmax > 0)
+    return rows_kv * kv * (key0 - 3 * own) >= (19ll << 20) / 10 && a->frac_bits <= (a->int_bits == 32 ? 28 : 38);
+  const int64_t wave = num_sms(), units = pl.items * pl.nchunk_max;
+  if (rows_kv > 128 && key0 < 512 && units > wave / 2 && units <= wave) return false;
+  if (own <= 256) {
+    if (rows_kv >= 4 || kv * cdiv(rows_kv, row_tile) * (key0 / attn::KT) <= 2 * wave) return true;
+  } else if (own > 4ll * key0 && units <= 3 * wave) {
+    return false;
+  }
+  return units > wave * (rows_kv < 4 ? 5 : rows_kv < 8 ? 3 : pl.rp == 16 ? 1 : 2);
 }
 
 struct PrefixPlan {
@@ -828,14 +862,13 @@ PrefixPlan prefix_plan_of(const fxpr_attention_params* a, int prefix_len, int64_
   int key0 = prefix_len < pl.max_keys ? prefix_len : pl.max_keys;
   key0 = key0 / attn::KT * attn::KT;  // the last keys of a ragged prefix run with each request's own
   const int64_t rows_kv = tokens * pl.G;
-  if ((a->head_dim != 64 && a->head_dim != 128) || !half(a->q_dtype) || !half(a->kv_dtype) ||
-      key0 < kPrefixMinKeys || a->num_blocks <= 0 ||
-      (pl.decode_kmax > 0 && rows_kv * a->num_kv_heads * key0 < kPrefixMinDecodePairs))
+  pp.row_tile = prefix_row_tile(rows_kv);
+  if ((a->head_dim != 64 && a->head_dim != 128) || !half(a->q_dtype) || !half(a->kv_dtype) || a->num_blocks <= 0 ||
+      !prefix_pays(a, pl, key0, pp.row_tile, rows_kv))
     return pp;
   auto fits = [](int64_t s) { return s >= 0 && s <= 0x7fffffffLL; };
   if (!fits(a->k_stride_blk) || !fits(a->k_stride_slot) || !fits(a->v_stride_blk) || !fits(a->v_stride_slot)) return pp;
   pp.key0 = key0;
-  pp.row_tile = prefix_row_tile(rows_kv);
   const int64_t tiles = cdiv(rows_kv, pp.row_tile);
   pp.nchunk = (int)cdiv(pl.max_keys - key0, attn::CHUNK);
   if (pp.nchunk < 1) pp.nchunk = 1;
@@ -956,11 +989,12 @@ extern "C" int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* a, 
   const PrefixPlan pp = prefix_plan_of(a, common_prefix_len, num_tokens);
   const int64_t nb = a->num_blocks;
   const Bounds bounds = {num_tokens, (int)(nb < 0 ? 0 : nb < INT32_MAX ? nb : INT32_MAX), 1};
-  if (!pp.use || a->workspace == nullptr) return run_unified(a, pp.pl, bounds, (cudaStream_t)stream);
-  if (a->workspace_bytes < pp.total || (uintptr_t)a->workspace % 256 != 0) {
-    set_error("shared_prefix_attention_fxp: the workspace must be 256-byte aligned and hold %lld bytes", (long long)pp.total);
+  const int64_t need = pp.use ? pp.total : pp.pl.total;
+  if (a->workspace != nullptr && (a->workspace_bytes < need || (uintptr_t)a->workspace % 256 != 0)) {
+    set_error("shared_prefix_attention_fxp: the workspace must be 256-byte aligned and hold %lld bytes", (long long)need);
     return FXPR_ERR_INVALID;
   }
+  if (!pp.use || a->workspace == nullptr) return run_unified(a, pp.pl, bounds, (cudaStream_t)stream);
   const Plan& pl = pp.pl;
   const cudaStream_t st = (cudaStream_t)stream;
   unsigned char* ws = reinterpret_cast<unsigned char*>(a->workspace);

@@ -136,3 +136,45 @@ def test_a_request_does_not_see_its_batch():
     far = torch.where(sl > 0, sl + 128, 0).int()
     large = _run(((q, torch.cat([kv, extra]), qsl, far, more), prefix + 128, mq, ms + 128), window_size=64)
     assert bits_equal(small, large)
+
+
+def _time(run):
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(4):
+            run()
+    best = float("inf")
+    for _ in range(6):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+# requests, queries of each, query heads, KV heads, head_dim, shared keys, own keys
+@pytest.mark.gpu
+@pytest.mark.parametrize("R, ql, H, KVH, D, prefix, own", [
+    (64, 1, 32, 8, 128, 1024, 3312), (64, 1, 32, 8, 128, 4096, 4096), (32, 1, 32, 8, 64, 2048, 4096), (16, 1, 32, 8, 128, 8192, 2048),
+    (2, 1, 8, 8, 128, 4096, 1024), (1, 1, 16, 8, 128, 8192, 512), (2, 1, 32, 32, 64, 2048, 2048), (4, 2, 32, 8, 128, 512, 4096),
+    (1, 1, 64, 8, 128, 4096, 1024), (24, 5, 32, 8, 64, 512, 2048), (64, 1, 16, 8, 128, 256, 1024),
+])
+def test_not_slower_than_unified_with_long_own_keys(R, ql, H, KVH, D, prefix, own):
+    """Own keys run in kernels that are slower than the unified attention's decode kernels, and behind more launches: where they are
+    many, the call takes the unified kernels (the rule that looked at the prefix alone took up to 2.4 times as long)."""
+    shared, each = prefix // PAGE, own // PAGE
+    bt = torch.empty(R, shared + each, dtype=torch.int32, device="cuda")
+    bt[:, :shared] = torch.arange(shared).int()
+    bt[:, shared:] = shared + torch.arange(R * each).int().view(R, each)
+    kv = torch.randn(shared + R * each, 2, PAGE, KVH, D, device="cuda").to(BF)
+    q = torch.randn(R * ql, H, D, device="cuda").to(BF)
+    qsl = (torch.arange(R + 1, device="cuda") * ql).int()
+    sl = torch.full((R,), prefix + own, dtype=torch.int32, device="cuda")
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+    new = _time(lambda: A.shared_prefix_attention_fxp(q, kv, a, qsl, sl, bt, prefix, ql, max_seq_len=prefix + own))
+    old = _time(lambda: A.unified_attention_fxp(q, kv, b, qsl, sl, bt, ql, frac_bits=16, max_seq_len=prefix + own))
+    assert bits_equal(a, b)
+    assert new < 1.1 * old, (new, old)

@@ -979,6 +979,13 @@ extern "C" int64_t fxpr_shared_prefix_attention_workspace_bytes(const fxpr_atten
   return pp.use ? pp.total : pp.pl.total;
 }
 
+extern "C" int fxpr_shared_prefix_attention_takes_prefix(const fxpr_attention_params* a, int common_prefix_len,
+                                                         int64_t num_tokens) {
+  if (validate_prefix(a, common_prefix_len, num_tokens) != FXPR_OK) return 0;
+  if (a->num_requests <= 0 || a->max_query_len <= 0 || num_tokens <= 0) return 0;
+  return prefix_plan_of(a, common_prefix_len, num_tokens).use ? 1 : 0;
+}
+
 extern "C" int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* a, int common_prefix_len,
                                                 int64_t num_tokens, void* stream) {
   int rc = validate_prefix(a, common_prefix_len, num_tokens);

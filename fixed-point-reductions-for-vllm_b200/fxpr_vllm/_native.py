@@ -37,6 +37,7 @@ EXPORTED = (
     "fxpr_gemm_fxp_noalloc", "fxpr_attention_workspace_bytes", "fxpr_fixed_to_float_add_rms_norm",
     "fxpr_qk_norm_rope_fxp", "fxpr_rope_append_kv_fxp",
     "fxpr_verify_draft_fxp", "fxpr_shared_prefix_attention_fxp", "fxpr_shared_prefix_attention_workspace_bytes",
+    "fxpr_shared_prefix_attention_takes_prefix",
 )
 
 _i = ctypes.c_int
@@ -114,6 +115,7 @@ _SIGS = {
     "fxpr_log_softmax_fxp": (_i, [_p, _i64, _p, _i64, _i64, _i64, _i, _i, _p]),
     "fxpr_shared_prefix_attention_fxp": (_i, [ctypes.POINTER(AttentionParams), _i, _i64, _p]),
     "fxpr_shared_prefix_attention_workspace_bytes": (_i64, [ctypes.POINTER(AttentionParams), _i, _i64]),
+    "fxpr_shared_prefix_attention_takes_prefix": (_i, [ctypes.POINTER(AttentionParams), _i, _i64]),
     "fxpr_qk_norm_rope_fxp": (_i, [ctypes.POINTER(RopeParams), _p]),
     "fxpr_rope_append_kv_fxp": (_i, [ctypes.POINTER(RopeParams), _p]),
     "fxpr_verify_draft_fxp": (_i, [_p, _p, _i, _i64, _i64, _i64, _i64, _p, _i, _p, _p, _i, _p, _p, _i64, _i, _i,

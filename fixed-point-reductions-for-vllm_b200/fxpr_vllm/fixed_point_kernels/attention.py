@@ -229,3 +229,43 @@ def shared_prefix_attention_fxp(
     rc = N.launch(lib.fxpr_shared_prefix_attention_fxp, dev, ctypes.byref(p), common_prefix_len, tokens)
     if rc:
         N.check(rc, what)
+
+
+def shared_prefix_takes_prefix_kernels(
+    common_prefix_len: int,
+    num_requests: int,
+    num_tokens: int,
+    max_query_len: int,
+    max_seq_len: int,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    page_size: int,
+    *,
+    dtype: torch.dtype = torch.bfloat16,
+    kv_dtype: torch.dtype | None = None,
+    fxp_dtype=torch.int32,
+    frac_bits: int = 16,
+    logits_soft_cap: float = 0.0,
+    window_size: int = 0,
+    alibi: bool = False,
+) -> bool:
+    """Whether :func:`shared_prefix_attention_fxp` runs the prefix kernels for
+    such a call (queries of ``dtype`` in rows of whole heads, a contiguous
+    cache), or else the unified attention's, with the same result. The
+    operator's own rule, asked on the host."""
+    p = N.AttentionParams()
+    p.q_dtype = p.o_dtype = N.DTYPE_CODE[dtype]
+    p.kv_dtype = N.DTYPE_CODE[dtype if kv_dtype is None else kv_dtype]
+    p.q_stride_tok = p.o_stride_tok = num_heads * head_dim
+    p.q_stride_head = p.o_stride_head = p.k_stride_head = p.v_stride_head = head_dim
+    p.k_stride_slot = p.v_stride_slot = num_kv_heads * head_dim
+    p.k_stride_blk = p.v_stride_blk = 2 * page_size * num_kv_heads * head_dim
+    p.num_requests, p.max_query_len, p.max_seq_len = num_requests, max_query_len, max_seq_len
+    p.num_heads, p.num_kv_heads, p.head_dim, p.page_size = num_heads, num_kv_heads, head_dim, page_size
+    p.block_table_cols = -(-max(max_seq_len, common_prefix_len) // page_size)
+    p.num_blocks = p.block_table_cols
+    p.is_causal, p.window_size, p.logits_soft_cap = 1, window_size, logits_soft_cap
+    p.alibi_slopes = 16 if alibi else None  # only whether they are given
+    p.frac_bits, p.int_bits = frac_bits, int_bits_of(fxp_dtype)
+    return bool(N.load().fxpr_shared_prefix_attention_takes_prefix(ctypes.byref(p), common_prefix_len, num_tokens))

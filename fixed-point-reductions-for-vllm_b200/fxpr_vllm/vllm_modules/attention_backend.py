@@ -24,7 +24,8 @@ import torch
 from vllm.v1.attention.backend import AttentionImpl, AttentionLayer, AttentionType
 from vllm.v1.attention.backends.triton_attn import TritonAttentionBackend, TritonAttentionMetadataBuilder
 
-from ..fixed_point_kernels.attention import shared_prefix_attention_fxp, unified_attention_fxp
+from ..fixed_point_kernels.attention import (shared_prefix_attention_fxp, shared_prefix_takes_prefix_kernels,
+                                              unified_attention_fxp)
 from ..fixed_point_kernels.fixed_point import RCP_LN2
 from ..fixed_point_kernels.rope import rope_append_kv_fxp
 from .config import get_runtime_config
@@ -33,25 +34,40 @@ logger = logging.getLogger("fxpr_vllm")
 
 
 class DeterministicAttentionMetadataBuilder(TritonAttentionMetadataBuilder):
-    """The Triton backend's metadata, with cascade attention for the steps that
-    the shared-prefix kernels take: a common prefix of ``MIN_PREFIX`` keys, and
-    ``MIN_DECODE_PAIRS`` (row, key) pairs where the decode kernels would run
-    otherwise (one query a request, four query heads a KV head). For the others
-    the operator runs the unified kernels, and the engine would only lose its
-    full CUDA graph."""
+    """The Triton backend's metadata, with cascade attention for the steps in
+    which the shared-prefix operator runs its prefix kernels, by the operator's
+    own rule. In the others it would run the unified kernels, and the engine
+    only lose its full CUDA graph. The engine does not say how many keys the
+    requests have behind the prefix: the rule is asked for the fewest possible
+    (their queries), and with many the operator runs the unified kernels after
+    all."""
 
-    MIN_PREFIX = 256
-    MIN_DECODE_PAIRS = 2 << 20
+    # of an instance: what its layers have
+    headdim = 128
+    block_size = 16
+    q_dtype = kv_dtype = torch.bfloat16
+    logits_soft_cap = 0.0
+
+    def __init__(self, kv_cache_spec, layer_names, vllm_config, device):
+        super().__init__(kv_cache_spec, layer_names, vllm_config, device)
+        self.headdim, self.kv_dtype = kv_cache_spec.head_size, kv_cache_spec.dtype
+        self.q_dtype = vllm_config.model_config.dtype
+        layers = vllm_config.compilation_config.static_forward_context
+        caps = [getattr(layers[n].impl, "logits_soft_cap", 0.0) for n in layer_names if n in layers]
+        self.logits_soft_cap = max(caps, default=0.0)
 
     def use_cascade_attention(self, common_prefix_len: int, query_lens, num_query_heads: int,
                               num_kv_heads: int, use_alibi: bool, use_sliding_window: bool,
                               use_local_attention: bool, num_sms: int, dcp_world_size: int) -> bool:
-        if (common_prefix_len < self.MIN_PREFIX or len(query_lens) < 2 or use_local_attention
-                or dcp_world_size > 1):
+        if len(query_lens) < 2 or use_local_attention or dcp_world_size > 1:
             return False
-        rows = int(sum(query_lens)) * num_query_heads
-        decode = max(query_lens) == 1 and num_query_heads == 4 * num_kv_heads
-        return not decode or rows * common_prefix_len >= self.MIN_DECODE_PAIRS
+        cfg = get_runtime_config()
+        prefix, longest = int(common_prefix_len), int(max(query_lens))
+        return shared_prefix_takes_prefix_kernels(
+            prefix, len(query_lens), int(sum(query_lens)), longest, prefix + longest, num_query_heads,
+            num_kv_heads, self.headdim, self.block_size, dtype=self.q_dtype, kv_dtype=self.kv_dtype,
+            fxp_dtype=cfg.fxp_int_bits, frac_bits=cfg.frac_bits, logits_soft_cap=self.logits_soft_cap,
+            window_size=int(use_sliding_window), alibi=bool(use_alibi))
 
     def build(self, common_prefix_len: int, common_attn_metadata, fast_build: bool = False):
         # the Triton builder's own cascade fields are not used (it leaves some

@@ -190,6 +190,11 @@ int64_t fxpr_attention_workspace_bytes(const fxpr_attention_params* p);
  * kernels. The workspace is 256-byte aligned, any contents. */
 int64_t fxpr_shared_prefix_attention_workspace_bytes(const fxpr_attention_params* p, int common_prefix_len,
                                                      int64_t num_tokens);
+/* 1 if such a call runs the prefix kernels, 0 if it runs the unified ones (or
+ * the parameters are invalid). Host only: sizes, types, strides and which
+ * optional inputs are given count, not what the pointers point to. */
+int fxpr_shared_prefix_attention_takes_prefix(const fxpr_attention_params* p, int common_prefix_len,
+                                              int64_t num_tokens);
 int fxpr_shared_prefix_attention_fxp(const fxpr_attention_params* p, int common_prefix_len, int64_t num_tokens,
                                      void* stream);
 

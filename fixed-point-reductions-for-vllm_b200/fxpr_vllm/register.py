@@ -125,6 +125,9 @@ def _log_config(cfg: FxpRuntimeConfig) -> None:
                 "gemm=%s attn=%s logprobs=%s", cfg.frac_bits, cfg.fxp_int_bits,
                 cfg.num_kv_splits, cfg.enable_rmsnorm, cfg.enable_gemm, cfg.enable_attn,
                 cfg.enable_logprobs)
+    if cfg.fused_rope:
+        logger.warning("VLLM_FXP_FUSED_ROPE has no effect: the engine keeps vLLM's rotary position. "
+                       "torch.ops.fxpr.rope_append_kv_fxp is there for code that calls it.")
 
 
 def register() -> None:

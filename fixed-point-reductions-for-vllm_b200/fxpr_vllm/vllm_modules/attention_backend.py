@@ -8,12 +8,14 @@ seq_lens, block_table, max_query_len, max_seq_len); the paged KV cache layout
 ``unified_attention_fxp`` on the B200 kernel, split over
 ``VLLM_FXP_NUM_KV_SPLITS`` KV splits (results do not depend on the count).
 
-Two additions to the reference's backend. When the engine's cascade attention
-is on (``disable_cascade_attn=False``) and all requests of a step share a
-prefix, ``shared_prefix_attention_fxp`` runs instead, with the same bits. With
-``VLLM_FXP_FUSED_ROPE=1`` the backend takes vLLM's fused rotary and cache
-update: the rotation then has one fixed arithmetic in every mode of the engine,
-where vLLM's own kernel and torch.compile's code round differently.
+An addition to the reference's backend: when the engine's cascade attention is
+on (``disable_cascade_attn=False``) and all requests of a step share a prefix,
+``shared_prefix_attention_fxp`` runs instead, with the same bits.
+
+The rotary position stays vLLM's in the engine. vLLM 0.22 fuses rotary and cache
+update on ROCm only, and there only for steps of up to 256 tokens, so offering
+it would give a token another rotation in a larger step. The method that it
+would call, ``do_rope_and_kv_cache_update``, is for callers of the layer itself.
 """
 
 from __future__ import annotations
@@ -131,7 +133,6 @@ class DeterministicAttentionImpl(AttentionImpl):
         self.frac_bits = cfg.frac_bits
         self.fxp_int_bits = cfg.fxp_int_bits
         self.num_kv_splits = cfg.num_kv_splits
-        self.fused_rope = cfg.fused_rope
         if alibi_slopes is not None:
             slopes = torch.tensor(alibi_slopes, dtype=torch.float32) * RCP_LN2
             assert slopes.shape == (num_heads,), \
@@ -184,14 +185,13 @@ class DeterministicAttentionImpl(AttentionImpl):
         reshape_and_cache_flash(key, value, key_cache, value_cache, slot_mapping,
                                 self.kv_cache_dtype, layer._k_scale, layer._v_scale)
 
-    def fused_rope_kvcache_supported(self) -> bool:
-        return self.fused_rope
-
     def do_rope_and_kv_cache_update(self, layer: AttentionLayer, query: torch.Tensor, key: torch.Tensor,
                                     value: torch.Tensor, positions: torch.Tensor,
                                     cos_sin_cache: torch.Tensor, is_neox: bool, kv_cache: torch.Tensor,
                                     layer_slot_mapping: torch.Tensor) -> None:
-        """Rotary position of query and key in place, key and value into the cache."""
+        """Rotary position of query and key in place, key and value into the
+        cache, for a caller that runs the layer itself: the engine does not
+        call it (``fused_rope_kvcache_supported`` stays false)."""
         n = query.shape[0]
         q = query.view(n, self.num_heads, self.head_size)
         k, v = (x.view(n, self.num_kv_heads, self.head_size) for x in (key, value))

@@ -69,7 +69,8 @@ _SWITCHES = {
     "enable_logprobs": "VLLM_FXP_DET_LOGPROBS",
     "enable_lm_head": "VLLM_FXP_DET_LM_HEAD",
 }
-# the same, default off
+# the same, default off. VLLM_FXP_FUSED_ROPE has no effect and is reported when
+# set: the engine's rotary position is vLLM's (see attention_backend.py).
 _OPT_INS = {
     "fused_rope": "VLLM_FXP_FUSED_ROPE",
 }

@@ -832,19 +832,20 @@ int prefix_row_tile(int64_t rows) {
 // shapes are then slower by more than 2%, the worst that several requests can
 // have by 21% (28.5 against 23.5 us); no shape loses more than 1.37 by the rule.
 constexpr int kPrefixMinKeys = 256;
+constexpr int64_t kWave = 148;  // CTAs; not asked of the device, so that the size query and the launch always agree
 bool prefix_pays(const fxpr_attention_params* a, const Plan& pl, int key0, int row_tile, int64_t rows_kv) {
   const int64_t own = pl.max_keys - key0, kv = a->num_kv_heads;
   if (key0 < kPrefixMinKeys) return false;
   if (pl.decode_kmax > 0)
     return rows_kv * kv * (key0 - 3 * own) >= (19ll << 20) / 10 && a->frac_bits <= (a->int_bits == 32 ? 28 : 38);
-  const int64_t wave = num_sms(), units = pl.items * pl.nchunk_max;
-  if (rows_kv > 128 && key0 < 512 && units > wave / 2 && units <= wave) return false;
+  const int64_t units = pl.items * pl.nchunk_max;
+  if (rows_kv > 128 && key0 < 512 && units > kWave / 2 && units <= kWave) return false;
   if (own <= 256) {
-    if (rows_kv >= 4 || kv * cdiv(rows_kv, row_tile) * (key0 / attn::KT) <= 2 * wave) return true;
-  } else if (own > 4ll * key0 && units <= 3 * wave) {
+    if (rows_kv >= 4 || kv * cdiv(rows_kv, row_tile) * (key0 / attn::KT) <= 2 * kWave) return true;
+  } else if (own > 4ll * key0 && units <= 3 * kWave) {
     return false;
   }
-  return units > wave * (rows_kv < 4 ? 5 : rows_kv < 8 ? 3 : pl.rp == 16 ? 1 : 2);
+  return units > kWave * (rows_kv < 4 ? 5 : rows_kv < 8 ? 3 : pl.rp == 16 ? 1 : 2);
 }
 
 struct PrefixPlan {

@@ -816,7 +816,10 @@ int prefix_row_tile(int64_t rows) {
 // one of 1008 shapes is then slower, by 2%. And not where most products
 // saturate: 64 requests behind 4096 keys, 28 fraction bits in 32-bit
 // accumulators 907 us against 1109, 30 bits 1186 against 1108; 38 bits in 64-bit
-// accumulators 941 against 1144, 40 bits 1262.
+// accumulators 941 against 1144, 40 bits 1262. Small batches with few own keys
+// keep the decode kernels: 8 requests behind 512 keys, own up to 64, take 23.9 us
+// here against 27.0 in a graph replay, but 33 against 31 us as calls, for the
+// three launches more; and steps with cascade attention are calls.
 //
 // Where it runs its chunk kernels, own keys cost the same in both forms, but
 // four launches wait for one another here instead of two. That shows while the

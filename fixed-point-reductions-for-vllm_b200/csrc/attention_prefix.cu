@@ -180,10 +180,11 @@ struct ScoresSmem {
   static constexpr size_t bytes = off_k + 2ull * KT64 * K_LD * 4;
 };
 // 2 CTAs per SM and 4 k-steps unrolled: 64 requests behind 4096 keys, 32 / 8
-// heads x 128, bf16 (1.07 G products): 84.4 us, 12.7 T products/s of the 18.4
-// that this tile's inner loop alone reaches; 3 CTAs 88.4 us (the 2048 units do
-// not divide as well), 16 k-steps 83.2 us here but 109.5 against 106.7 us with
-// head_dim 64.
+// heads x 128, bf16 (1.07 G products): 86 us, 12.5 T products/s of the 18.4 that
+// this tile's inner loop alone reaches. The rest: 26% more instructions, 5% less
+// issued while an SM has work, and 11% of the cycles in which one has none
+// (start, tail). 3 CTAs 3 us more (the 2048 units do not divide as well), 16
+// k-steps 1 us less here but 3 us more with head_dim 64.
 constexpr int SCORES_CTAS = 2;
 constexpr int SU = 4;
 constexpr int BD = 16;  // dims of a block that is rounded one way
@@ -507,8 +508,9 @@ struct PvSmem {
   static constexpr size_t off_p = 2 * v_buf;
   static constexpr size_t bytes = off_p + 2 * p_buf;
 };
-// At the sizes above 122.4 us, 8.8 T products/s of the 12.5 of the inner loop
-// alone; 16 k-steps unrolled 132 us.
+// At the sizes above 125 us, 8.6 T products/s of the 12.5 of the inner loop
+// alone (21% more instructions, 4% less issued, 14% of the cycles without work);
+// 16 k-steps unrolled 8 us more.
 constexpr int VU_UNROLL = 4;
 
 template <int D, int RT, int BITS, typename T>

@@ -14,9 +14,10 @@
 // norm and rotation as two operators round twice.
 //
 // Bound: HBM. Each row is read and written once. 8192 tokens, 32 + 8 heads x
-// 128, bf16: rotation and append 35.8 us for 204 MB (5.7 TB/s, 87% of a copy);
-// with the norm 34.4 us for 170 MB (4.9 TB/s, 76%): there 250 instructions a
-// lane and row keep the issue slots half busy as well.
+// 128, bf16: rotation and append 35.6 us for 204 MB (5.7 TB/s, 88% of a copy;
+// 49% of the issue slots); with the norm 34.1 us for 170 MB (5.0 TB/s, 76%):
+// there 250 instructions a lane and row take 70% of the issue slots, and neither
+// side is full.
 //
 // Layout of the vector kernel: a row belongs to a group of LPR lanes and each
 // lane holds two 8-value pieces, chosen so that both halves of a rotation pair

@@ -31,10 +31,12 @@ namespace fxpr {
 namespace verify {
 
 // 256 threads, six CTAs per SM (40 registers), four 16-byte loads per tensor
-// of a lane in flight: 128 requests of 128256 fp32 entries, 81 of them refusing
-// (83 MB), 21.4 us (3.9 TB/s, 59% of a copy; about 8 us of it are the launch,
-// the chain of reads that decides on the drafted tokens, and the draw). Four or
-// five CTAs 2 to 3 us more, 512 threads 3 us. One request: 3.8 us.
+// of a lane in flight: 128 requests of 128256 fp32 entries, 81 to 94 of them
+// refusing (89 MB), 21.5 us (4.2 TB/s, 64% of a copy). In the same batch 3.6 us
+// if none refuses (launch and the chain of reads that decides on the drafted
+// tokens), 30.9 us if all do (131 MB, 4.3 TB/s); one request that refuses 6.8 us;
+// a refusing request more costs 0.2 us (5.1 TB/s). Four or five CTAs 2 to 3 us
+// more, 512 threads 3 us. One request, its drafts taken two times in three: 3.9 us.
 constexpr int THREADS = 256;
 constexpr int MINB = 6;
 constexpr int UNROLL = 4;

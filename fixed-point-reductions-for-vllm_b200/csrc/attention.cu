@@ -163,8 +163,7 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
     const int j = kb + ti * KT + my_jl;
     if (j >= ke) return -1;
     const int bi = p.page_shift >= 0 ? (j >> p.page_shift) : j / p.page;
-    const int b = p.bt[bt_row + bi];
-    return b < p.blocks ? b : -1;
+    return p.bt[bt_row + bi];
   };
   auto issue = [&](const void* base, int64_t sb, int64_t ss, int64_t sh, int ti, int b, int blk) {
     const int c0 = (t % TPK) * CPT;
@@ -172,7 +171,8 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
     unsigned char* dst = kvbuf + b * TILEB + my_jl * ROWB;
     const unsigned char* src = reinterpret_cast<const unsigned char*>(base);
     int bytes = 0;
-    if (blk >= 0) {
+    // checked here, not in block_of: there it would wait for the block-table read
+    if ((unsigned)blk < (unsigned)p.blocks) {
       const int slot = p.page_shift >= 0 ? (j & (p.page - 1)) : j % p.page;
       src += ((int64_t)blk * sb + (int64_t)slot * ss + (int64_t)kvh * sh) * (int64_t)sizeof(KVT);
       bytes = 16;
@@ -371,6 +371,7 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
   if (t < RP) {
     float m = -INFINITY;
     for (int q = 0; q < nsplit; ++q) m = fmaxf(m, *cluster.map_shared_rank(&rmax_s[t], q));
+    if (p.skip_masked && m == -INFINITY) m = 0.0f;  // no key: p = exp2(-inf) = 0
     gmax_s[t] = m;  // == the reference's pass-1 max over the whole context
   }
   __syncthreads();
@@ -435,12 +436,8 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
       float pv = 0.0f;
       if (j < ke) {
         const float sc = recompute ? S_tmp[prow * KT + jl] : S[prow * (p.cap + 8) + ti * KT + jl];
-        if (p.skip_masked && sc == -INFINITY) {
-          pv = -0.0f;
-        } else {
-          pv = prim_exp2(__fsub_rn(sc, gm));
-          if (j < kend_p) den_acc += (UAcc)f2x_f32<BITS>(pv, scale);
-        }
+        pv = prim_exp2(__fsub_rn(sc, gm));
+        if (j < kend_p) den_acc += (UAcc)f2x_f32<BITS>(pv, scale);
       }
       // key slot: the KPT keys of PV thread group kg are contiguous
       P[prow * KT + (jl % KG) * KPT + jl / KG] = __fmul_rn(pv, scale);
@@ -509,7 +506,9 @@ __global__ void __launch_bounds__(THREADS) attn_kernel(Params p) {
         for (int i = 0; i < RP; ++i) {
           if (j >= row_kend[i]) continue;
           const float ps = P[i * KT + kg * KPT + u];
-          if (__float_as_uint(ps) == 0x80000000u) continue;  // masked (exp2 gives no -0)
+          if (p.skip_masked &&
+              (recompute ? S_tmp[i * KT + jl] : S[i * (p.cap + 8) + ti * KT + jl]) == -INFINITY)
+            continue;
           const auto x0 = f2x_scaled<BITS>(__fmul_rn(ps, vv.x));
           const auto x1 = f2x_scaled<BITS>(__fmul_rn(ps, vv.y));
           if constexpr (BITS == 64) {

@@ -122,8 +122,7 @@ struct TileCopier {
     const int j = kb + ti * NK + my_jl;
     if (j >= ke) return -1;
     const int bi = p.page_shift >= 0 ? (j >> p.page_shift) : j / p.page;
-    const int b = p.bt[bt_row + bi];
-    return b < p.blocks ? b : -1;
+    return p.bt[bt_row + bi];
   }
   __device__ __forceinline__ void issue(const void* base, int64_t sb, int64_t ss, int64_t sh,
                                         int ti, unsigned char* dst_tile, int blk) const {
@@ -131,7 +130,8 @@ struct TileCopier {
     unsigned char* dst = dst_tile + my_jl * TL::ROWB;
     const unsigned char* src = reinterpret_cast<const unsigned char*>(base);
     int bytes = 0;
-    if (blk >= 0) {
+    // checked here, not in block_of: there it would wait for the block-table read
+    if ((unsigned)blk < (unsigned)p.blocks) {
       const int slot = p.page_shift >= 0 ? (j & (p.page - 1)) : j % p.page;
       src += ((int64_t)blk * sb + (int64_t)slot * ss + (int64_t)kvh * sh) * (int64_t)sizeof(KVT);
       bytes = 16;
@@ -640,8 +640,10 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_scores_rq_kernel(Params p) {
 // kernel 2: normaliser, PV and the integer combine
 // ---------------------------------------------------------------------------
 // PRE: over the keys from p.key0 on; the row maxima are complete, the sums of
-// the keys before are in the row accumulators.
-template <int D, int RP, int BITS, typename KVT, bool PRE = false>
+// the keys before are in the row accumulators. SKIP: a masked key (score -inf)
+// is kept as p = -0 and contributes nothing whatever its V holds; a form of its
+// own, for the choice at run time slowed 16-row units by 1 to 3%.
+template <int D, int RP, int BITS, typename KVT, bool PRE = false, bool SKIP = PRE>
 __global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_kernel(Params p) {
   constexpr int NBP = PRE ? NBP_PRE : attn::NBP;
   using TL = Tile<D, KVT>;
@@ -732,7 +734,7 @@ __global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_ker
     const int j = kb + k;
     float pv = 0.0f;
     UAcc den = 0;
-    if ((PRE || p.skip_masked) && (j >= ke || P_all[i * CHUNK + k] == -INFINITY)) {
+    if (SKIP && (j >= ke || P_all[i * CHUNK + k] == -INFINITY)) {
       pv = -0.0f;
     } else if (j < ke) {
       pv = prim_exp2(__fsub_rn(P_all[i * CHUNK + k], gmax_s[i]));
@@ -852,7 +854,7 @@ __global__ void __launch_bounds__(THREADS, suffix_pv_ctas(PRE, RP)) chunk_pv_ker
         for (int i = 0; i < RP; ++i) {
           if (j >= row_kend[i]) continue;
           const float ps = Pk[i * CHUNK + u];
-          if (__float_as_uint(ps) == 0x80000000u) continue;  // masked (exp2 gives no -0)
+          if (SKIP && __float_as_uint(ps) == 0x80000000u) continue;
           const auto x0 = f2x_scaled<BITS>(__fmul_rn(ps, vv.x));
           const auto x1 = f2x_scaled<BITS>(__fmul_rn(ps, vv.y));
           if constexpr (BITS == 64) {
@@ -976,11 +978,12 @@ static int launch_chunked_t(const Params& p, int req, int ys, cudaStream_t st) {
   } else {
     k1 = plain ? chunk_scores_kernel<D, RP, BITS, KVT, true> : chunk_scores_kernel<D, RP, BITS, KVT, false>;
   }
-  void (*k2)(Params) = chunk_pv_kernel<D, RP, BITS, KVT>;
-  static bool done1[2][64] = {{false}}, done2[64] = {false};
+  void (*k2)(Params) =
+      p.skip_masked ? chunk_pv_kernel<D, RP, BITS, KVT, false, true> : chunk_pv_kernel<D, RP, BITS, KVT>;
+  static bool done1[2][64] = {{false}}, done2[2][64] = {{false}};
   int rc = configure((const void*)k1, s1, done1[plain ? 1 : 0]);
   if (rc != FXPR_OK) return rc;
-  rc = configure((const void*)k2, s2, done2);
+  rc = configure((const void*)k2, s2, done2[p.skip_masked ? 1 : 0]);
   if (rc != FXPR_OK) return rc;
   const dim3 grid((unsigned)p.nchunk_max, (unsigned)ys, (unsigned)((int64_t)req * p.qtiles));
   k1<<<grid, THREADS, s1, st>>>(p);

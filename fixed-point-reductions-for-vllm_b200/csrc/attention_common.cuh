@@ -51,10 +51,10 @@ struct Params {
   // [0, blocks) reads zeros
   int64_t tokens;
   int blocks;
-  // the shared-prefix operator: a masked key (score -inf) has p = -0, which
-  // contributes nothing whatever its V holds, and a row of only such keys is 0.
-  // The unified attention computes p = exp2(-inf - max) as the reference does:
-  // the clamp turns 0 * inf and a row of NaN into the smallest integer.
+  // the shared-prefix operator: a masked key (score -inf) contributes nothing
+  // whatever its V holds, and a row of only such keys is 0. The unified
+  // attention computes p = exp2(-inf - max) and p * V as the reference does: the
+  // clamp turns 0 * inf and a row of NaN into the smallest integer.
   int skip_masked;
   // chunked path: caller workspace (no state between calls)
   uint32_t* ws_cnt;            // [items] chunks finished

@@ -803,7 +803,7 @@ int prefix_row_tile(int64_t rows) {
 }
 
 // Whether the prefix kernels are the faster form. Device time of the unified
-// attention over theirs (above 1: they win), 3863 shapes, graph replays, bf16,
+// attention over theirs (above 1: they win), graph replays of 6767 shapes, bf16,
 // uniform requests; "own" are the keys behind the prefix.
 //
 // Where the unified attention runs its decode kernels (one query a request,
@@ -825,14 +825,15 @@ int prefix_row_tile(int64_t rows) {
 // unified attention's units (512 keys of an item) do not fill the GPU: 8 / 8
 // heads behind 8192 keys, one request, own 16 0.64, 1024 0.41; four requests
 // 2.03, 1.32; 16 requests 6.7, 3.8; 64 / 8 heads behind 1024 keys, one request,
-// own 64 2.4, 1024 0.9. Hence taken with up to 256 own keys, if a tile has rows
-// to share K with (four a KV head) or the prefix kernels' units are resident at
-// once; and with more where those units exceed 1 wave of CTAs (16-row units), 2
-// (4-row units), 3 (below 8 rows a KV head) or 5 (below 4). Not below 512 prefix
-// keys with many rows and half a wave to a wave of units (0.75 to 1), nor with
-// own keys more than four times the prefix up to 3 waves (0.8 to 1). 57 of 2855
-// shapes are then slower by more than 2%, the worst that several requests can
-// have by 21% (28.5 against 23.5 us); no shape loses more than 1.37 by the rule.
+// own 64 2.4, 1024 0.9. Hence taken with up to 384 own keys (256 for 4-row units
+// of fewer than 8 rows a KV head), if a tile has rows to share K with (four a KV
+// head) or the prefix kernels' units are resident at once; and with more where
+// the unified attention's units exceed 1 wave of CTAs (16-row units), 2 (4-row
+// units), 3 (below 8 rows a KV head) or 5 (below 4). Not below 320 prefix keys
+// with many rows and nearly a wave of units (0.75 to 1), nor with own keys more
+// than four times the prefix up to 3 waves (0.8 to 1). 129 of 5759 shapes are then
+// slower by more than 2%, 36 by more than 10%, the worst by 30% (24.5 against
+// 18.9 us); where the rule takes the unified kernels it loses 37% at most.
 constexpr int kPrefixMinKeys = 256;
 constexpr int64_t kWave = 148;  // CTAs; not asked of the device, so that the size query and the launch always agree
 bool prefix_pays(const fxpr_attention_params* a, const Plan& pl, int key0, int row_tile, int64_t rows_kv) {
@@ -841,8 +842,8 @@ bool prefix_pays(const fxpr_attention_params* a, const Plan& pl, int key0, int r
   if (pl.decode_kmax > 0)
     return rows_kv * kv * (key0 - 3 * own) >= (19ll << 20) / 10 && a->frac_bits <= (a->int_bits == 32 ? 28 : 38);
   const int64_t units = pl.items * pl.nchunk_max;
-  if (rows_kv > 128 && key0 < 512 && units > kWave / 2 && units <= kWave) return false;
-  if (own <= 256) {
+  if (rows_kv > 128 && key0 < 320 && units > 3 * kWave / 4 && units <= kWave) return false;
+  if (own <= (rows_kv >= 8 || pl.rp == 16 ? 384 : 256)) {
     if (rows_kv >= 4 || kv * cdiv(rows_kv, row_tile) * (key0 / attn::KT) <= 2 * kWave) return true;
   } else if (own > 4ll * key0 && units <= 3 * kWave) {
     return false;
